@@ -350,6 +350,63 @@ int pe_adamw_step(int dtype, int64_t n, void* p, const void* g, float* m, float*
  * ------------------------------------------------------------------------- */
 int pe_wait_probe(uint64_t limit_ns, int32_t* status, int32_t* waited_out, void* stream);
 
+/* ------------------------------------------------ the drafter's key/value cache ----
+ * Keys and values of all requests lie in pages of one pool, k_cache / v_cache
+ * [num_pages, Hkv, page, hd] (contiguous); request b's key t lies in page
+ * table[b * table_ld + t / page] at offset t % page.  The reference keeps no drafter
+ * cache: every draft runs the drafter over its whole context (drafter.py:195-236).
+ *
+ * pe_cache_plan takes request b (B <= 8192) from lens[b] to new_lens[b] cached keys.  The
+ * free pages are a ring of num_pages entries, ring[0] (head) and ring[1] (tail) counting
+ * pages taken and given back so far: free page i of tail - head is
+ * free_ring[(head + i) % num_pages].  In request order, growth takes pages from the head
+ * into the block table (up to `width` pages a row), shrinking pushes pages onto the tail;
+ * pages given back in a call are not taken in it.  The first `shared` keys (whole pages)
+ * of every request belong to a shared prefix whose pages are neither taken nor given back.
+ *   granted[b]  new_lens[b], or lens[b] when the request is refused: lengths that are
+ *               negative or beyond the table, growth once the pages run out (all later
+ *               growth with it), pages given back that the ring has no room for
+ *   cu[B + 1]   first new row of each request (max(0, new_lens - lens) rows each)
+ *   slots/pos   per new row, `rows` of them: slot (page * page_size + offset; -1 for a
+ *               refused request's rows and rows behind cu[B]) and position (0 behind cu[B])
+ *   ring_out[3] head and tail after the call, and how many requests were refused
+ * table and free_ring are updated in place; ring_out and granted must not alias inputs. */
+int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_t page, int64_t rows,
+                  int64_t shared, const int32_t* lens, const int32_t* new_lens, int32_t* table,
+                  int64_t table_ld, int32_t* free_ring, const int64_t* ring, int64_t* ring_out,
+                  int32_t* granted, int32_t* cu, int64_t* slots, int64_t* pos, void* stream);
+
+/* Copy row t of k and v ([rows, Hkv * hd], row strides k_ld, v_ld) into cache slot slots[t];
+ * rows with a slot outside [0, num_pages * page) are skipped.  Two rows with the same slot
+ * leave either one's values. */
+int pe_cache_append(int dtype, int64_t rows, int Hkv, int hd, const void* k, int64_t k_ld,
+                    const void* v, int64_t v_ld, const int64_t* slots, int64_t num_pages,
+                    int64_t page, void* k_cache, void* v_cache, void* stream);
+
+/* Attention of the new rows q [T, Hq * hd] of B requests over their cached keys: request b
+ * owns rows cu[b] .. cu[b + 1], lens[b] counts its keys with the new rows among them, and
+ * its row j sees keys t < lens[b] - n_b + j + 1 (prediction slots follow the last real row,
+ * so this is the attend rule of masks.py:43-61 for one anchor).  A row that sees no key
+ * gives o = 0, lse = -inf; rows behind cu[B] are left as they were.  lse: fp32 [Hq, T],
+ * natural log.  Head sizes 1..256, Hq / Hkv <= 256, pages of a multiple of 16 keys.
+ *
+ * shared > 0 (whole pages): the first `shared` keys of every request are those of table row
+ * 0; they are read once for all rows, and the requests' own keys joined to them.  Every
+ * request with rows must then hold the prefix: lens[b] - n_b >= shared.
+ *
+ * What a cache holds behind a request's keys does not matter (NaN included); keys below
+ * lens[b] are finite, or the rows of the tile that masks them may turn NaN too.  Block table
+ * entries outside the pool read as zero keys and values.  workspace:
+ * pe_attn_paged_workspace bytes, 256-byte aligned, for this call alone while it runs. */
+size_t pe_attn_paged_workspace(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd,
+                               int64_t shared);
+int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd, const void* q,
+                  int64_t q_ld, const void* k_cache, const void* v_cache, int64_t num_pages,
+                  int64_t page, const int32_t* table, int64_t table_ld, int64_t width,
+                  const int32_t* lens, const int32_t* cu, int64_t shared, void* o, int64_t o_ld,
+                  float* lse, void* workspace, size_t workspace_bytes, int algo, int* status,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

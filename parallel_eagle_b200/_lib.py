@@ -104,6 +104,19 @@ SIGNATURES: dict[str, tuple] = {
     "pe_adamw_step": (
         _int, [_int, _i64, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _f32, _f32, _i64, _vp]
     ),
+    "pe_cache_plan": (
+        _int, [_i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+               _vp, _vp, _vp]
+    ),
+    "pe_cache_append": (
+        _int, [_int, _i64, _int, _int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp]
+    ),
+    "pe_attn_paged_workspace": (_sz, [_int, _i64, _i64, _int, _int, _int, _i64]),
+    "pe_attn_paged": (
+        _int,
+        [_int, _i64, _i64, _int, _int, _int, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
+         _vp, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _int, _vp, _vp],
+    ),
     "pe_wait_probe": (_int, [C.c_uint64, _vp, _vp, _vp]),
 }
 

@@ -1,0 +1,313 @@
+// The drafter's paged key/value cache: the page plan (block tables, slot maps, pages
+// taken from and given back to the free ring) and the append of new rows.
+//
+// The cache itself is [pages, Hkv, page, hd] for K and for V: one head's keys of one page
+// are contiguous, so the attention kernels read whole pages with single copies.  The
+// reference keeps no drafter cache: it runs the drafter over the whole context for every
+// draft (src/pe/drafter.py:195-236).
+#include <limits.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace pe {
+namespace {
+
+// ---------------------------------------------------------------- page plan ----
+// Request b goes from lens[b] cached keys to new_lens[b].  With used = ceil(len / page) and
+// need = ceil(new_len / page) pages (neither below the shared ones), need - used pages are
+// taken from the ring's head, or used - need are pushed onto its tail, in request order; the
+// new rows new_len - len get their positions and slots (page * page_size + offset).
+//
+// Every block scans all requests by itself (they are a few KB that sit in L2) and then takes
+// its share of the three flat index spaces -- new rows, pages taken, pages given back --
+// finding an index's request by bisection in shared memory.  A row's page comes straight
+// from the ring when this call is the one that takes it, so no block reads what another
+// writes and one launch does it all.  Bound by launch latency up to some 100K rows, by the
+// 16 bytes written per row above.
+constexpr int kPlanThreads = 512;
+constexpr int kPlanBatch = 8192;  // requests whose scan fits the block's shared memory
+
+struct Scan3 {
+  int64_t rows;
+  int grow, drop;
+};
+
+__device__ __forceinline__ Scan3 add3(Scan3 a, Scan3 b) {
+  return {a.rows + b.rows, a.grow + b.grow, a.drop + b.drop};
+}
+
+// last index i in [0, n) with v[i] <= x (v ascending, v[0] = 0)
+__device__ __forceinline__ int find(const int* v, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
+            const int32_t* __restrict__ lens, const int32_t* __restrict__ want,
+            int32_t* table, int64_t table_ld, int32_t* ring_pages,
+            const int64_t* __restrict__ ring, int64_t* __restrict__ ring_out,
+            int32_t* __restrict__ granted, int32_t* __restrict__ cu, int64_t* __restrict__ slots,
+            int64_t* __restrict__ pos) {
+  extern __shared__ int sm[];
+  int* s_cu = sm;                  // [B + 1] first new row
+  int* s_grow = s_cu + B + 1;      // [B + 1] pages taken by the requests before
+  int* s_drop = s_grow + B + 1;    // [B + 1] pages given back by the requests before
+  __shared__ Scan3 s_warp[kPlanThreads / 32];
+  __shared__ int s_refused, s_taken, s_given;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_refused = s_taken = s_given = 0;
+  const int64_t head = ring[0], tail = ring[1];
+  // counters that no ring of N pages can have serve nothing
+  const bool sane = head >= 0 && tail >= head && tail - head <= N;
+  const int64_t avail = sane ? tail - head : 0, room = sane ? N - avail : 0;
+
+  // used / need of request b; false when the lengths are not served by the table at all
+  auto pages_of = [&](int b, int& from, int& to, int& used, int& need) {
+    from = lens[b];
+    to = want[b];
+    const bool fits = from >= 0 && to >= 0 && (to + (int64_t)page - 1) / page <= width &&
+                      (from + (int64_t)page - 1) / page <= width;
+    used = fits ? max((int)(((int64_t)from + page - 1) / page), sp) : 0;
+    need = fits ? max((int)(((int64_t)to + page - 1) / page), sp) : 0;
+    return fits;
+  };
+
+  // ---- exclusive scan of (new rows, pages taken, pages given back) over the requests ----
+  Scan3 carry{0, 0, 0};
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    Scan3 v{0, 0, 0};
+    int from = 0, to = 0, used = 0, need = 0;
+    if (b < B) {
+      pages_of(b, from, to, used, need);
+      // (lengths the table cannot hold still own their rows, without slots)
+      v.rows = max((int64_t)0, (int64_t)to - from);
+      v.grow = max(0, need - used);
+      v.drop = max(0, used - need);
+    }
+    Scan3 inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const Scan3 t{__shfl_up_sync(0xffffffffu, inc.rows, o), __shfl_up_sync(0xffffffffu, inc.grow, o),
+                    __shfl_up_sync(0xffffffffu, inc.drop, o)};
+      if (lane >= o) inc = add3(inc, t);
+    }
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    Scan3 base = carry;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) base = add3(base, s_warp[w]);
+      carry = add3(carry, s_warp[w]);
+    }
+    if (b < B) {
+      s_cu[b] = (int)min(base.rows + inc.rows - v.rows, (int64_t)INT_MAX);  // (only wild lengths)
+      s_grow[b] = base.grow + inc.grow - v.grow;
+      s_drop[b] = base.drop + inc.drop - v.drop;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    s_cu[B] = (int)min(carry.rows, (int64_t)INT_MAX);
+    s_grow[B] = carry.grow;
+    s_drop[B] = carry.drop;
+  }
+  __syncthreads();
+
+  // a request is served when its pages are there: growth while the ring's pages last,
+  // returns while the ring has room (it always has, unless a page was given back twice)
+  auto served = [&](int b, bool fits) {
+    const bool grows = s_grow[b + 1] > s_grow[b], drops = s_drop[b + 1] > s_drop[b];
+    return fits && (!grows || s_grow[b + 1] <= avail) && (!drops || s_drop[b + 1] <= room);
+  };
+
+  if (blockIdx.x == 0) {
+    for (int b = tid; b < B; b += kPlanThreads) {
+      int from, to, used, need;
+      const bool ok = served(b, pages_of(b, from, to, used, need));
+      granted[b] = ok ? to : from;
+      if (ok && need > used) atomicAdd(&s_taken, need - used);
+      if (ok && used > need) atomicAdd(&s_given, used - need);
+      if (!ok) atomicAdd(&s_refused, 1);
+    }
+    for (int b = tid; b <= B; b += kPlanThreads) cu[b] = s_cu[b];
+    __syncthreads();
+    if (tid == 0) {
+      ring_out[0] = head + s_taken;
+      ring_out[1] = tail + s_given;
+      ring_out[2] = s_refused;
+    }
+  }
+
+  const int64_t stride = (int64_t)gridDim.x * kPlanThreads, i0 = (int64_t)blockIdx.x * kPlanThreads + tid;
+  // ---- new rows: position and slot ----
+  for (int64_t r = i0; r < rows; r += stride) {
+    int64_t slot = -1, p = 0;
+    if (r < s_cu[B]) {
+      const int b = find(s_cu, B, (int)r);
+      int from, to, used, need;
+      const bool ok = served(b, pages_of(b, from, to, used, need));
+      p = (int64_t)from + (int)r - s_cu[b];
+      if (ok) {
+        const int64_t i = p / page;
+        const int id = i >= used ? ring_pages[(head + s_grow[b] + i - used) % N]
+                                 : table[(int64_t)b * table_ld + i];
+        slot = (int64_t)id * page + p % page;
+      }
+    }
+    slots[r] = slot;
+    pos[r] = p;
+  }
+  // ---- pages taken: table entries ----
+  for (int64_t g = i0; g < min((int64_t)s_grow[B], avail); g += stride) {
+    const int b = find(s_grow, B, (int)g);
+    int from, to, used, need;
+    if (!served(b, pages_of(b, from, to, used, need))) continue;
+    table[(int64_t)b * table_ld + used + (int)g - s_grow[b]] = ring_pages[(head + g) % N];
+  }
+  // ---- pages given back: ring entries ----
+  for (int64_t d = i0; d < min((int64_t)s_drop[B], room); d += stride) {
+    const int b = find(s_drop, B, (int)d);
+    int from, to, used, need;
+    if (!served(b, pages_of(b, from, to, used, need))) continue;
+    ring_pages[(tail + d) % N] = table[(int64_t)b * table_ld + need + (int)d - s_drop[b]];
+  }
+}
+
+// ------------------------------------------------------------------- append ----
+// Row t of k / v -> its slot in the cache: per head a contiguous run of hd elements.  A
+// copy, bound by HBM: one read and one write of each row.  A thread moves kItems pieces
+// of K and of V (16 bytes each when rows and cache allow it), with all of its loads
+// issued before the first store.
+constexpr int kAppendThreads = 256;
+constexpr int kItems = 4;
+
+// I: the type that holds every index (32-bit divisions where the sizes allow them).
+template <typename V, typename I>
+__global__ void __launch_bounds__(kAppendThreads)
+append_kernel(int64_t rows, int per_row, int per_head, int Hkv, const V* __restrict__ k,
+              int64_t k_ld, const V* __restrict__ v, int64_t v_ld,
+              const int64_t* __restrict__ slots, int64_t num_slots, int page, V* __restrict__ kc,
+              V* __restrict__ vc) {
+  const I total = (I)rows * per_row;
+  const I base = (I)blockIdx.x * (kAppendThreads * kItems) + threadIdx.x;
+  V kv[kItems], vv[kItems];
+  int64_t dst[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const I at = base + (I)(i * kAppendThreads);
+    dst[i] = -1;
+    if (at >= total) continue;
+    const I row = at / (I)per_row;
+    const uint32_t j = (uint32_t)(at - row * (I)per_row);
+    const int64_t slot = slots[row];
+    if (slot < 0 || slot >= num_slots) continue;
+    const uint32_t h = j / (uint32_t)per_head;
+    const I pg = (I)slot / (I)page;
+    const uint32_t off = (uint32_t)((I)slot - pg * (I)page);
+    dst[i] = (((int64_t)pg * Hkv + h) * page + off) * per_head + (j - h * (uint32_t)per_head);
+    kv[i] = k[(int64_t)row * k_ld + j];
+    vv[i] = v[(int64_t)row * v_ld + j];
+  }
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    if (dst[i] < 0) continue;
+    kc[dst[i]] = kv[i];
+    vc[dst[i]] = vv[i];
+  }
+}
+
+template <typename V>
+int append_launch(int64_t rows, int Hkv, int hd_units, const void* k, int64_t k_ld, const void* v,
+                  int64_t v_ld, const int64_t* slots, int64_t num_slots, int page, void* kc,
+                  void* vc, cudaStream_t st) {
+  const int per_row = Hkv * hd_units;
+  const int64_t blocks = ceil_div(rows * per_row, kAppendThreads * kItems);
+  PE_CHECK_ARG(blocks < (1ll << 31), "cache_append: too many rows for one launch");
+  // (the last block's indices run past the total by less than a block)
+  const bool small = num_slots < (1ll << 31) &&
+                     rows * per_row < (1ll << 32) - kAppendThreads * kItems;
+  auto kern = small ? append_kernel<V, uint32_t> : append_kernel<V, uint64_t>;
+  kern<<<(unsigned)blocks, kAppendThreads, 0, st>>>(
+      rows, per_row, hd_units, Hkv, (const V*)k, k_ld, (const V*)v, v_ld, slots, num_slots, page,
+      (V*)kc, (V*)vc);
+  PE_LAUNCHED();
+  return PE_OK;
+}
+
+}  // namespace
+}  // namespace pe
+
+using namespace pe;
+
+extern "C" int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_t page,
+                             int64_t rows, int64_t shared, const int32_t* lens,
+                             const int32_t* new_lens, int32_t* table, int64_t table_ld,
+                             int32_t* free_ring, const int64_t* ring, int64_t* ring_out,
+                             int32_t* granted, int32_t* cu, int64_t* slots, int64_t* pos,
+                             void* stream) {
+  PE_CHECK_ARG(B >= 1 && B <= kPlanBatch, "cache_plan: %lld requests, expected 1 to %d",
+               (long long)B, kPlanBatch);
+  PE_CHECK_ARG(page >= 1 && page <= (1 << 20), "cache_plan: page size %lld", (long long)page);
+  PE_CHECK_ARG(width >= 1 && width * page < (1ll << 31) && table_ld >= width,
+               "cache_plan: block table of %lld pages (row stride %lld)", (long long)width,
+               (long long)table_ld);
+  PE_CHECK_ARG(num_pages >= 1 && num_pages < (1ll << 31) && B * width < (1ll << 31),
+               "cache_plan: %lld pages", (long long)num_pages);
+  PE_CHECK_ARG(rows >= 0 && rows < (1ll << 31), "cache_plan: %lld new rows", (long long)rows);
+  PE_CHECK_ARG(shared >= 0 && shared % page == 0 && shared / page <= width,
+               "cache_plan: %lld shared keys are not whole pages of the table", (long long)shared);
+  PE_CHECK_ARG(lens && new_lens && table && free_ring && ring && ring_out && granted && cu &&
+                   (rows == 0 || (slots && pos)),
+               "cache_plan: null pointer");
+  PE_CHECK_ARG(ring != ring_out && lens != granted && new_lens != granted,
+               "cache_plan: ring_out and granted must not alias the inputs");
+  const size_t smem = 3 * (size_t)(B + 1) * sizeof(int);
+  if (smem > 48 * 1024)
+    PE_CUDA_TRY(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)smem));
+  // a block per 1024 rows (and per 256 requests, whose pages it fills), up to one per SM
+  const int64_t want = std::max(ceil_div(rows, 2 * kPlanThreads), ceil_div(B, 256));
+  const int blocks = (int)std::min<int64_t>(std::max<int64_t>(want, 1), sm_count());
+  plan_kernel<<<blocks, kPlanThreads, smem, as_stream(stream)>>>(
+      (int)B, width, num_pages, (int)page, rows, (int)(shared / page), lens, new_lens, table,
+      table_ld, free_ring, ring, ring_out, granted, cu, slots, pos);
+  PE_LAUNCHED();
+  return PE_OK;
+}
+
+extern "C" int pe_cache_append(int dtype, int64_t rows, int Hkv, int hd, const void* k,
+                               int64_t k_ld, const void* v, int64_t v_ld, const int64_t* slots,
+                               int64_t num_pages, int64_t page, void* k_cache, void* v_cache,
+                               void* stream) {
+  PE_CHECK_ARG(dtype == PE_F32 || dtype == PE_BF16, "cache_append: unsupported dtype code %d",
+               dtype);
+  PE_CHECK_ARG(rows >= 0 && Hkv >= 1 && hd >= 1 && (int64_t)Hkv * hd < (1 << 24),
+               "cache_append: %lld rows of %d heads of %d", (long long)rows, Hkv, hd);
+  PE_CHECK_ARG(num_pages >= 0 && page >= 1 && page <= (1 << 20), "cache_append: %lld pages of %lld",
+               (long long)num_pages, (long long)page);
+  if (rows == 0) return PE_OK;
+  PE_CHECK_ARG(k && v && slots && k_cache && v_cache, "cache_append: null pointer");
+  PE_CHECK_ARG(rows == 1 || (k_ld >= (int64_t)Hkv * hd && v_ld >= (int64_t)Hkv * hd),
+               "cache_append: row strides %lld, %lld below %d x %d", (long long)k_ld,
+               (long long)v_ld, Hkv, hd);
+  const int es = dtype == PE_F32 ? 4 : 2, per16 = 16 / es;
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  const bool wide = hd % per16 == 0 && k_ld % per16 == 0 && v_ld % per16 == 0 && al(k) && al(v) &&
+                    al(k_cache) && al(v_cache);
+  const cudaStream_t st = as_stream(stream);
+  if (wide)
+    return append_launch<uint4>(rows, Hkv, hd / per16, k, k_ld / per16, v, v_ld / per16, slots,
+                                num_pages * page, (int)page, k_cache, v_cache, st);
+  if (es == 4)
+    return append_launch<uint32_t>(rows, Hkv, hd, k, k_ld, v, v_ld, slots, num_pages * page,
+                                   (int)page, k_cache, v_cache, st);
+  return append_launch<uint16_t>(rows, Hkv, hd, k, k_ld, v, v_ld, slots, num_pages * page,
+                                 (int)page, k_cache, v_cache, st);
+}

@@ -1,0 +1,264 @@
+// Attention that reads the paged key/value cache: the pieces its kernels share.
+//
+// The work of one launch is a line of cost units: request after request, within a request
+// KV head after KV head, within a head one entity per tile of Mt query rows (a row is one
+// (new token, query head of the KV head's group) pair; rows of a group share their keys, so
+// packing them fills the matrix instructions' row dimension).  An entity's cost is about
+// its keys.  Each block takes an equal piece of that line, so a batch of any raggedness
+// loads all SMs alike, a lone long request is split over all of them, and no host knowledge
+// of the lengths is needed: a block finds its piece from lens and cu alone.
+//
+// A piece that is a whole entity writes its rows' result.  Otherwise an entity's pieces
+// leave partial results (accumulator, running maximum, sum) in per-block slots -- a block
+// has at most two incomplete entities, its first and its last -- and the block that holds
+// the entity's first piece records how many there are; the combine kernel joins them in
+// piece order, so results do not depend on timing.
+#pragma once
+#include "common.cuh"
+
+namespace pe {
+namespace paged {
+
+struct Args {
+  const void* q;          // [T, Hq * hd], row stride q_ld
+  int64_t q_ld;
+  const void *kc, *vc;    // [num_pages, Hkv, page, hd]
+  int64_t num_pages;
+  int page;
+  const int32_t* table;   // [B, width] (row stride table_ld)
+  int64_t table_ld;
+  int64_t kmax;           // keys a table row can hold: width * page
+  const int32_t* lens;    // [B] keys of each request, its new rows among them
+  const int32_t* cu;      // [B + 1] first row of each request
+  int B, T, Hq, Hkv, hd, G;  // G = Hq / Hkv
+  int64_t kbeg;           // first key (the shared prefix, when another launch does it)
+  int all_rows;           // 1: one request of cu[B] rows that all see keys [kbeg, kmax)
+  float scale_log2;       // log2(e) / sqrt(hd)
+  void* o;                // result rows (the operand type), row stride o_ld
+  int64_t o_ld;
+  float* lse;             // [Hq, T]
+  float* o32;             // when set, results go here instead (fp32 [T, Hq, hd]) with lse
+  const float* pre_o;     // a prefix's result [T, Hq, hd] and lse [Hq, T] to join with
+  const float* pre_lse;
+  float* part_o;          // [2 * blocks, Mt, hd] unnormalised accumulators
+  float* part_ml;         // [2 * blocks, Mt, 2] running maximum (log2 units) and sum
+  struct Open* open;      // [blocks] incomplete entity that starts in the block
+  int* status;
+};
+
+// an entity whose first piece block c holds and whose rest the blocks after it hold
+struct Open {
+  int parts;   // 0: none
+  int slot;    // first piece's slot; piece i > 0 lies in slot 2 * (c + i)
+  int row0;    // first row of the request
+  int r0;      // first packed row (token * G + head in group) of the tile
+  int rows;    // packed rows of the tile
+  int kvh;
+  int pad[2];
+};
+
+constexpr float kLn2f = 0.6931471805599453f;
+
+// one request as a launch sees it
+struct Req {
+  int row0, n;        // first row in q, new rows
+  int64_t first;      // keys row 0 sees, kbeg included (row j sees first + j; all_rows: constant)
+  int R;              // row tiles
+  int64_t A;          // cost model: (A + slope terms), see cost()
+};
+
+template <int Mt, int TK>
+struct Sched {
+  const Args& a;
+  int64_t total, per, pos, end;  // cost units; this block's piece is [pos, end)
+  int b;                         // request that holds pos
+  int64_t base;                  // its first unit
+  Req rq;
+  // the current segment: entity (rq, kvh, rt), key tiles [t0, t1) of nt
+  int kvh, rt, t0, t1, nt;
+  bool first, last;
+  int64_t kend;                  // keys the entity's last row sees (exclusive end)
+  int seg;                       // segments taken so far
+
+  __device__ __forceinline__ Sched(const Args& args) : a(args) {}
+
+  __device__ __forceinline__ int requests() const { return a.all_rows ? 1 : a.B; }
+
+  __device__ __forceinline__ Req request(int i) const {
+    Req r;
+    if (a.all_rows) {
+      r.row0 = 0;
+      r.n = max(0, min(a.cu[a.B], a.T));
+      r.first = a.kmax;
+      r.A = a.kmax - a.kbeg;
+    } else {
+      const int c0 = a.cu[i], c1 = a.cu[i + 1];
+      r.row0 = max(0, min(c0, a.T));
+      r.n = max(0, min(c1, a.T) - r.row0);
+      r.first = (int64_t)a.lens[i] - ((int64_t)c1 - c0) + 1;
+      r.A = max((int64_t)0, min(r.first, a.kmax) - a.kbeg);
+    }
+    r.R = (int)(((int64_t)r.n * a.G + Mt - 1) / Mt);
+    return r;
+  }
+  // cost of row tile rt: its keys times G, plus a key tile's worth for its start and end
+  __device__ __forceinline__ int64_t cost(const Req& r, int rt) const {
+    return (r.A + TK) * a.G + (a.all_rows ? 0 : (int64_t)(rt + 1) * Mt);
+  }
+  __device__ __forceinline__ int64_t cost_before(const Req& r, int64_t rt) const {
+    return rt * (r.A + TK) * a.G + (a.all_rows ? 0 : rt * (rt + 1) / 2 * Mt);
+  }
+  __device__ __forceinline__ int64_t req_cost(const Req& r) const {
+    return (int64_t)a.Hkv * cost_before(r, r.R);
+  }
+
+  // all threads of the block; scratch: one int64 per warp plus 4
+  __device__ __forceinline__ void init(int64_t* scratch) {
+    const int n = requests(), tid = threadIdx.x, nthr = blockDim.x;
+    const int lane = tid & 31, warp = tid >> 5, nw = nthr >> 5;
+    const int chunk = (n + nthr - 1) / nthr;
+    const int i0 = min(n, tid * chunk), i1 = min(n, i0 + chunk);
+    int64_t mine = 0;
+    for (int i = i0; i < i1; ++i) mine += req_cost(request(i));
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    if (tid == 0) scratch[nw] = -1;
+    __syncthreads();
+    int64_t before = inc - mine, sum = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) before += scratch[w];
+      sum += scratch[w];
+    }
+    total = sum;
+    // an equal share each, but no piece below two key tiles' work
+    per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)3 * TK * a.G);
+    pos = min(total, (int64_t)blockIdx.x * per);
+    end = min(total, pos + per);
+    // the thread whose requests hold pos finds the request
+    if (pos < end && before <= pos && pos < before + mine) {
+      int i = i0;
+      int64_t at = before;
+      while (true) {
+        const int64_t c = req_cost(request(i));
+        if (pos < at + c) break;
+        at += c;
+        ++i;
+      }
+      scratch[nw] = i;
+      scratch[nw + 1] = at;
+    }
+    __syncthreads();
+    b = (int)scratch[nw];
+    base = scratch[nw + 1];
+    seg = 0;
+    if (pos < end) rq = request(b);
+    __syncthreads();
+  }
+
+  // next segment of the piece; false when there is none.  Same result in every thread.
+  __device__ __forceinline__ bool next() {
+    if (pos >= end) return false;
+    int64_t rc = req_cost(rq);
+    while (pos >= base + rc) {  // (requests without rows cost nothing)
+      base += rc;
+      rq = request(++b);
+      rc = req_cost(rq);
+    }
+    const int64_t head_cost = cost_before(rq, rq.R);
+    int64_t off = pos - base;
+    kvh = (int)(off / head_cost);
+    off -= kvh * head_cost;
+    // last row tile that starts at or before off
+    int lo = 0, hi = rq.R;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cost_before(rq, mid) <= off) lo = mid; else hi = mid;
+    }
+    rt = lo;
+    const int64_t c = cost(rq, rt), u0 = off - cost_before(rq, rt);
+    const int64_t u1 = min(c, u0 + (end - pos));
+    // the entity's key tiles, in proportion to its units
+    const int rows_end = (int)min((int64_t)rq.n * a.G, (int64_t)(rt + 1) * Mt);
+    const int last_tok = (rows_end - 1) / a.G;
+    kend = min(a.kmax, a.all_rows ? a.kmax : rq.first + last_tok);
+    nt = kend > a.kbeg ? (int)((kend - a.kbeg + TK - 1) / TK) : 0;
+    first = u0 == 0;
+    last = u1 == c;
+    t0 = first ? 0 : (int)(u0 * nt / c);
+    t1 = last ? nt : (int)(u1 * nt / c);
+    entity_end_ = pos - u0 + c;
+    pos += u1 - u0;
+    ++seg;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return first && last; }
+  // slot of the current (incomplete) segment's partial result
+  __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (seg == 1 ? 0 : 1); }
+  // pieces of the current entity, for the block that holds its first piece but not its last
+  __device__ __forceinline__ int parts() const {
+    return (int)((entity_end_ - 1) / per) - (int)blockIdx.x + 1;
+  }
+  // keys that packed row r (of the whole request) sees, as an exclusive end
+  __device__ __forceinline__ int64_t limit(int r) const {
+    return min(a.kmax, a.all_rows ? a.kmax : rq.first + r / a.G);
+  }
+  __device__ __forceinline__ int tile_rows() const {
+    return (int)min((int64_t)Mt, (int64_t)rq.n * a.G - (int64_t)rt * Mt);
+  }
+  // block table row of the current request
+  __device__ __forceinline__ const int32_t* pages() const {
+    return a.table + (a.all_rows ? 0 : (int64_t)b * a.table_ld);
+  }
+  // recorded by one thread for a segment that is its entity's first piece but not all of it
+  __device__ __forceinline__ void record_open() const {
+    Open r{};
+    r.parts = parts();
+    r.slot = slot();
+    r.row0 = rq.row0;
+    r.r0 = rt * Mt;
+    r.rows = tile_rows();
+    r.kvh = kvh;
+    a.open[blockIdx.x] = r;
+  }
+
+ private:
+  int64_t entity_end_;
+};
+
+// What a finished row's accumulator is multiplied by: o = own * acc + pre * pre_o.
+struct RowScale {
+  float own, pre, lse;
+};
+
+// m (log2 units) and l: running maximum and sum over the row's keys; t, head: the row
+__device__ __forceinline__ RowScale finish_row(const Args& a, int t, int head, float m, float l) {
+  RowScale s;
+  if (!a.pre_lse) {
+    s.own = l == 0.f ? 0.f : 1.f / l;
+    s.pre = 0.f;
+    s.lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2f;
+    return s;
+  }
+  const float own = l == 0.f ? -INFINITY : m + log2f(l);
+  const float pre = a.pre_lse[(int64_t)head * a.T + t] * (1.f / kLn2f);
+  const float top = fmaxf(own, pre);
+  if (top == -INFINITY) {
+    s.own = s.pre = 0.f;
+    s.lse = -INFINITY;
+    return s;
+  }
+  const float wo = exp2f(own - top), wp = exp2f(pre - top), w = wo + wp;
+  s.own = l == 0.f ? 0.f : wo / (w * l);
+  s.pre = pre == -INFINITY ? 0.f : wp / w;
+  s.lse = (top + log2f(w)) * kLn2f;
+  return s;
+}
+
+
+}  // namespace paged
+}  // namespace pe

@@ -449,6 +449,164 @@ def attn_bwd_segments(q, k, v, o, do, lse, n_heads, n_kv_heads, head_dim, bounds
     return dq, dk, dv
 
 
+# ----------------------------------------------------- key/value cache ----
+
+
+def _same_device(*ts: torch.Tensor) -> torch.device:
+    """The device all operands are on, which has to be the current one (a kernel
+    launched for another device's memory would run on the current device's stream)."""
+    L.require_cuda(*ts)
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise L.PeError(f"operands on {dev} and {t.device}: one device is needed")
+    if dev.index != torch.cuda.current_device():
+        raise L.PeError(f"operands on {dev}, but the current device is "
+                        f"cuda:{torch.cuda.current_device()} (use torch.cuda.device)")
+    return dev
+
+
+def _ints(what: str, t: torch.Tensor, n: int | None, dtype: torch.dtype) -> None:
+    if t.dim() != 1 or t.dtype != dtype or not t.is_contiguous() or n not in (None, t.shape[0]):
+        want = "" if n is None else f"[{n}] "
+        raise L.PeError(f"{what} must be a contiguous {want}{dtype} vector, got "
+                        f"{tuple(t.shape)} {t.dtype}")
+
+
+def _block_table(what: str, table: torch.Tensor, batch: int) -> None:
+    if (table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != batch
+            or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1)):
+        raise L.PeError(f"{what}: the block table must be int32 [{batch}, pages] with unit column "
+                        f"stride, got {tuple(table.shape)} {table.dtype}")
+
+
+def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
+    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous() or 0 in k_cache.shape):
+        raise L.PeError(f"{what}: the caches must be two contiguous [pages, kv heads, page, "
+                        f"head_dim] tensors of one dtype, got {tuple(k_cache.shape)} "
+                        f"{k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
+    return tuple(k_cache.shape)
+
+
+def cache_plan(lens, new_lens, table, free, ring, page: int, rows: int, *, shared: int = 0,
+               ring_out=None):
+    """Plan the pages of a batch of requests that go from ``lens`` to ``new_lens`` cached
+    keys (int32 ``[B]``): new rows, prediction slots and prompts grow a request, rejected
+    drafts and finished requests shrink it.  Pages come from and go back to the free ring
+    (``free`` int32 ``[pages]``, ``ring`` int64 ``[3]``: head, tail, -) in request order;
+    ``table`` (int32 ``[B, width]``) and ``free`` are updated in place.  ``rows`` is the
+    number of new rows (the host knows what it submits; rows beyond them get slot -1).
+
+    Returns ``(granted, cu, slots, pos, ring_out)``: the lengths now held (``lens`` where a
+    request was refused), the first new row of each request (int32 ``[B + 1]``), each new
+    row's cache slot and position (int64 ``[rows]``) and the ring after the call, whose last
+    entry counts refused requests.  The first ``shared`` keys (whole pages) of all requests
+    belong to a shared prefix and are left alone."""
+    if ring_out is None:
+        ring_out = torch.empty_like(ring)
+    dev = _same_device(lens, new_lens, table, free, ring, ring_out)
+    batch = lens.shape[0] if lens.dim() == 1 else -1
+    _ints("cache_plan: lens", lens, batch, torch.int32)
+    _ints("cache_plan: new_lens", new_lens, batch, torch.int32)
+    _ints("cache_plan: free", free, None, torch.int32)
+    _ints("cache_plan: ring", ring, 3, torch.int64)
+    _ints("cache_plan: ring_out", ring_out, 3, torch.int64)
+    _block_table("cache_plan", table, batch)
+    # slots and pos, then granted and cu, from one allocation each
+    rows = int(rows)
+    if rows < 0:
+        raise L.PeError(f"cache_plan: {rows} new rows")
+    per_row = torch.empty(2, rows, dtype=torch.int64, device=dev)
+    per_req = torch.empty(2 * batch + 1, dtype=torch.int32, device=dev)
+    granted, cu = per_req[:batch], per_req[batch:]
+    rc = _lib().pe_cache_plan(
+        batch, table.shape[1], free.shape[0], int(page), rows, int(shared), lens.data_ptr(),
+        new_lens.data_ptr(), table.data_ptr(), _row_stride(table), free.data_ptr(),
+        ring.data_ptr(), ring_out.data_ptr(), granted.data_ptr(), cu.data_ptr(),
+        per_row.data_ptr(), per_row.data_ptr() + 8 * rows, L.stream_ptr(dev),
+    )
+    L.check(rc, "pe_cache_plan")
+    return granted, cu, per_row[0], per_row[1], ring_out
+
+
+def cache_append(k, v, slots, k_cache, v_cache) -> None:
+    """Write row t of ``k`` and ``v`` (``[rows, kv heads * head_dim]`` row views, keys already
+    rotated) into slot ``slots[t]`` (int64) of the caches; rows whose slot lies outside the
+    cache (-1) are skipped.  Slots of one call are distinct, as :func:`cache_plan` gives them."""
+    dev = _same_device(k, v, slots, k_cache, v_cache)
+    pages, hkv, page, hd = _caches("cache_append", k_cache, v_cache)
+    if (k.dim() != 2 or k.shape != v.shape or k.shape[1] != hkv * hd
+            or k.dtype != k_cache.dtype or v.dtype != k_cache.dtype):
+        raise L.PeError(f"cache_append: k and v must be {k_cache.dtype} [rows, {hkv * hd}], got "
+                        f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    _ints("cache_append: slots", slots, k.shape[0], torch.int64)
+    rc = _lib().pe_cache_append(
+        L.dtype_code(k.dtype), k.shape[0], hkv, hd, k.data_ptr(), _row_stride(k), v.data_ptr(),
+        _row_stride(v), slots.data_ptr(), pages, page, k_cache.data_ptr(), v_cache.data_ptr(),
+        L.stream_ptr(dev),
+    )
+    L.check(rc, "pe_cache_append")
+
+
+def attn_paged(q, k_cache, v_cache, table, lens, cu, o=None, lse=None, algo=L.ALGO_AUTO):
+    """Attention of the new rows of a batch of requests over their cached keys.  ``q`` (a
+    ``[T, heads * head_dim]`` row view) holds request b's rows at ``cu[b] .. cu[b + 1]``
+    (int32 ``[B + 1]``); ``lens[b]`` (int32) counts its keys, the new rows' (appended before
+    the call) among them, and its row j sees the keys below ``lens[b] - n_b + j + 1``.  One
+    row per request is a decode step, ``max_depth`` rows a draft, more a prompt in chunks.
+
+    Returns ``(o, lse)``: ``o`` like ``q`` and fp32 ``lse`` ``[heads, T]``.  Rows behind
+    ``cu[B]`` are not written; a row that sees no key gives 0 and ``-inf``."""
+    return _attn_paged(q, k_cache, v_cache, table, lens, cu, 0, o, lse, algo)
+
+
+def attn_paged_shared(q, k_cache, v_cache, table, lens, cu, shared: int, o=None, lse=None,
+                      algo=L.ALGO_AUTO):
+    """:func:`attn_paged` for requests whose first ``shared`` keys (whole pages) are the same
+    pages -- samples or drafts forked from one prompt.  The prefix is taken from ``table[0]``
+    and read once for all rows; ``lens`` counts it.  Every request with rows holds the whole
+    prefix (``lens[b] - n_b >= shared``)."""
+    if int(shared) < 0:
+        raise L.PeError(f"attn_paged_shared: {shared} shared keys")
+    return _attn_paged(q, k_cache, v_cache, table, lens, cu, int(shared), o, lse, algo)
+
+
+def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
+    dev = _same_device(q, k_cache, v_cache, table, lens, cu, o, lse)
+    pages, hkv, page, hd = _caches("attn_paged", k_cache, v_cache)
+    if q.dim() != 2 or q.dtype != k_cache.dtype or q.shape[1] % (hkv * hd) or q.shape[1] == 0:
+        raise L.PeError(f"attn_paged: q must be {k_cache.dtype} [rows, heads * {hd}] with heads a "
+                        f"multiple of {hkv}, got {tuple(q.shape)} {q.dtype}")
+    batch = lens.shape[0] if lens.dim() == 1 else -1
+    _ints("attn_paged: lens", lens, batch, torch.int32)
+    _ints("attn_paged: cu", cu, batch + 1, torch.int32)
+    _block_table("attn_paged", table, batch)
+    T, heads = q.shape[0], q.shape[1] // hd
+    if o is None:
+        o = torch.empty(T, heads * hd, dtype=q.dtype, device=dev)
+    elif o.shape != q.shape or o.dtype != q.dtype:
+        raise L.PeError(f"attn_paged: o must be like q, got {tuple(o.shape)} {o.dtype}")
+    if lse is None:
+        lse = torch.empty(heads, T, dtype=torch.float32, device=dev)
+    elif lse.shape != (heads, T) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise L.PeError(f"attn_paged: lse must be contiguous float32 [{heads}, {T}]")
+    lib = _lib()
+    code = L.dtype_code(q.dtype)
+    nbytes = int(lib.pe_attn_paged_workspace(code, batch, T, heads, hkv, hd, shared))
+    # the call's own scratch, from torch's stream-ordered allocator: calls on other streams
+    # and captured graphs never share it
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    rc = lib.pe_attn_paged(
+        code, batch, T, heads, hkv, hd, q.data_ptr(), _row_stride(q), k_cache.data_ptr(),
+        v_cache.data_ptr(), pages, page, table.data_ptr(), _row_stride(table), table.shape[1],
+        lens.data_ptr(), cu.data_ptr(), shared, o.data_ptr(), _row_stride(o), lse.data_ptr(),
+        ws.data_ptr(), nbytes, algo, status_word(dev).data_ptr(), L.stream_ptr(dev),
+    )
+    L.check(rc, "pe_attn_paged")
+    return o, lse
+
+
 def topk_logprobs(logits: torch.Tensor, k: int, raw: bool = False):
     """``(values, indices)`` of the ``k`` largest log-softmax entries of every row of
     ``logits`` ``[rows, V]`` (fp32 log-probabilities, int64 columns), ordered by value

@@ -1,0 +1,95 @@
+"""Host-side checks of the paged cache entry points: argument validation happens before any
+CUDA call, and the wrappers refuse host tensors (no GPU needed)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from parallel_eagle_b200 import _lib, ops
+
+BF16, F32, F16 = 1, 0, 2
+
+
+def _plan(lib, B=1, width=4, pages=8, page=16, rows=3, shared=0, table_ld=4, p=1):
+    p = p or None
+    # distinct non-null addresses that are never dereferenced on the host
+    return lib.pe_cache_plan(B, width, pages, page, rows, shared, p, p, p, table_ld, p, p,
+                             p and p + 64, p and p + 128, p, p, p, None)
+
+
+def test_plan_validates():
+    lib = _lib.load()
+    for kw in (dict(B=0), dict(B=8193), dict(page=0), dict(width=0), dict(table_ld=3),
+               dict(pages=0), dict(rows=-1), dict(shared=-16), dict(shared=8), dict(shared=80),
+               dict(width=1 << 28, table_ld=1 << 28), dict(p=0)):
+        assert _plan(lib, **kw) == 1, kw
+        assert b"cache_plan" in lib.pe_last_error()
+    # outputs that alias the inputs they are computed from
+    assert lib.pe_cache_plan(1, 4, 8, 16, 3, 0, 1, 1, 1, 4, 1, 1, 1, 129, 1, 1, 1, None) == 1
+    assert b"alias" in lib.pe_last_error()
+
+
+def _append(lib, dtype=BF16, rows=4, Hkv=2, hd=64, k_ld=128, v_ld=128, pages=4, page=16, p=16):
+    p = p or None
+    return lib.pe_cache_append(dtype, rows, Hkv, hd, p, k_ld, p, v_ld, p, pages, page, p, p, None)
+
+
+def test_append_validates():
+    lib = _lib.load()
+    for kw in (dict(dtype=F16), dict(rows=-1), dict(Hkv=0), dict(hd=0), dict(k_ld=127),
+               dict(v_ld=64), dict(pages=-1), dict(page=0), dict(p=0)):
+        assert _append(lib, **kw) == 1, kw
+        assert b"cache_append" in lib.pe_last_error()
+    assert _append(lib, rows=0, p=0) == 0
+
+
+def _attn(lib, dtype=BF16, B=2, T=4, Hq=4, Hkv=2, hd=64, q_ld=256, pages=8, page=16, table_ld=4,
+          width=4, shared=0, o_ld=256, ws=256, nbytes=1 << 40, algo=0, p=16):
+    p = p or None
+    return lib.pe_attn_paged(dtype, B, T, Hq, Hkv, hd, p, q_ld, p, p, pages, page, p, table_ld,
+                             width, p, p, shared, p, o_ld, p, ws, nbytes, algo, None, None)
+
+
+def test_attention_validates():
+    lib = _lib.load()
+    for kw in (dict(dtype=F16), dict(Hq=3), dict(Hq=0), dict(Hkv=0), dict(Hq=514, Hkv=2),
+               dict(hd=0), dict(hd=257), dict(B=0), dict(T=-1), dict(T=1 << 30), dict(page=8),
+               dict(page=24), dict(pages=0), dict(width=0), dict(width=1 << 27, table_ld=1 << 27),
+               dict(table_ld=3), dict(shared=-16), dict(shared=8), dict(shared=80), dict(q_ld=255),
+               dict(o_ld=128), dict(algo=7), dict(p=0)):
+        assert _attn(lib, **kw) == 1, kw
+        assert b"attn_paged" in lib.pe_last_error()
+    # a workspace that is missing, short or misaligned
+    for kw in (dict(ws=None), dict(nbytes=16), dict(ws=264)):
+        assert _attn(lib, **kw) == 4, kw
+        assert b"workspace" in lib.pe_last_error()
+    assert _attn(lib, T=0, p=0) == 0
+
+
+def test_workspace_sizes():
+    lib = _lib.load()
+    own = lib.pe_attn_paged_workspace(BF16, 8, 40, 28, 4, 128, 0)
+    assert own > 0
+    # a shared prefix adds its rows' fp32 result
+    assert lib.pe_attn_paged_workspace(BF16, 8, 40, 28, 4, 128, 64) >= own + 40 * 28 * 129 * 4
+    assert lib.pe_attn_paged_workspace(BF16, 0, 40, 28, 4, 128, 0) == 0
+    assert lib.pe_attn_paged_workspace(BF16, 8, 0, 28, 4, 128, 0) == 0
+
+
+def test_wrappers_refuse_host_tensors():
+    i = torch.zeros(2, dtype=torch.int32)
+    table = torch.zeros(2, 3, dtype=torch.int32)
+    cache = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    rows = torch.zeros(2, 128, dtype=torch.bfloat16)
+    ring = torch.zeros(3, dtype=torch.int64)
+    calls = [
+        lambda: ops.cache_plan(i, i, table, i, ring, 16, 2),
+        lambda: ops.cache_append(rows, rows, torch.zeros(2, dtype=torch.int64), cache, cache),
+        lambda: ops.attn_paged(rows, cache, cache, table, i, torch.zeros(3, dtype=torch.int32)),
+        lambda: ops.attn_paged_shared(rows, cache, cache, table, i,
+                                      torch.zeros(3, dtype=torch.int32), 16),
+    ]
+    for call in calls:
+        with pytest.raises(_lib.PeError, match="CUDA tensors only"):
+            call()
