@@ -301,15 +301,28 @@ int launch_simt(int dtype, const Args& a, int blocks, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ kernel choice ----
-enum Kind { kSimt };
+enum Kind { kSimt, kFew };
 
 struct Phase {
   Kind kind;
   int Mt, blocks;
 };
 
-Phase choose(int dtype, int hd) {
-  return {kSimt, kSimtRows, sm_count() * (hd <= 128 ? 4 : 2)};
+Phase simt_phase(int hd) { return {kSimt, kSimtRows, sm_count() * (hd <= 128 ? 4 : 2)}; }
+
+// tensor-core kernel for `rows` packed rows (on average) per request and KV head
+Phase tc_phase(int64_t rows) {
+  const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return {kFew, n, sm_count()};
+}
+
+bool tc_sizes(int dtype, int hd) { return dtype == PE_BF16 && (hd == 64 || hd == 128); }
+
+// whether the tensor-core kernels take the call's operands
+bool tc_operands(const Args& a) {
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  return al(a.q) && a.q_ld % 8 == 0 && al(a.kc) && al(a.vc) &&
+         a.num_pages * a.Hkv * a.page < (1ll << 31) - 256;
 }
 
 int64_t al256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -329,7 +342,8 @@ void carve(Args& a, const Phase& p, uint8_t* ws) {
 }
 
 int run_phase(int dtype, const Phase& p, const Args& a, cudaStream_t st) {
-  int rc = launch_simt(dtype, a, p.blocks, st);
+  const int rc = p.kind == kFew ? launch_few(a, p.Mt, p.blocks, st)
+                                : launch_simt(dtype, a, p.blocks, st);
   if (rc) return rc;
   return launch_join(dtype, a, p.blocks, p.Mt, st);
 }
@@ -344,10 +358,12 @@ using namespace pe::paged;
 extern "C" size_t pe_attn_paged_workspace(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd,
                                           int64_t shared) {
   if (B < 1 || T < 1 || Hq < 1 || Hkv < 1 || hd < 1) return 0;
-  const int64_t own = phase_bytes(choose(dtype, hd), hd);
-  if (shared <= 0) return (size_t)own;
-  const int64_t pre = al256(T * Hq * hd * 4) + al256(T * Hq * 4);
-  return (size_t)(pre + std::max(own, phase_bytes(choose(dtype, hd), hd)));
+  const int64_t G = std::max(Hq / Hkv, 1);
+  int64_t bytes = phase_bytes(simt_phase(hd), hd);  // (operands may rule the tensor cores out)
+  if (tc_sizes(dtype, hd)) bytes = std::max(bytes, phase_bytes(tc_phase(ceil_div(T * G, B)), hd));
+  if (shared <= 0) return (size_t)bytes;
+  if (tc_sizes(dtype, hd)) bytes = std::max(bytes, phase_bytes(tc_phase(T * G), hd));
+  return (size_t)(al256(T * Hq * hd * 4) + al256(T * Hq * 4) + bytes);
 }
 
 extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd,
@@ -395,6 +411,12 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
   a.B = (int)B; a.T = (int)T; a.Hq = Hq; a.Hkv = Hkv; a.hd = hd; a.G = Hq / Hkv;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
   a.o = o; a.o_ld = o_ld; a.lse = lse; a.status = status;
+  const bool tc = algo != PE_ALGO_SIMT && tc_sizes(dtype, hd) && tc_operands(a);
+  if (algo == PE_ALGO_TCGEN05 && !tc) {
+    set_error("attn_paged: the tensor-core kernels take bf16, head_dim 64 or 128, 16-byte aligned "
+              "rows and pools below 2^31 keys x heads");
+    return PE_ERR_UNSUPPORTED;
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (shared > 0) {
     // the prefix once, all rows of all requests together, into fp32 rows
@@ -402,7 +424,7 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     ws += al256(T * Hq * hd * 4);
     float* pre_lse = reinterpret_cast<float*>(ws);
     ws += al256(T * Hq * 4);
-    const Phase p = choose(dtype, hd);
+    const Phase p = tc ? tc_phase(T * a.G) : simt_phase(hd);
     Args pa = a;
     pa.all_rows = 1;
     pa.kmax = shared;
@@ -415,7 +437,7 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     a.pre_o = pre_o;
     a.pre_lse = pre_lse;
   }
-  const Phase p = choose(dtype, hd);
+  const Phase p = tc ? tc_phase(ceil_div(T * a.G, B)) : simt_phase(hd);
   carve(a, p, ws);
   return run_phase(dtype, p, a, st);
 }

@@ -260,5 +260,9 @@ __device__ __forceinline__ RowScale finish_row(const Args& a, int t, int head, f
 }
 
 
+// Tensor-core kernels (bf16, head sizes 64 and 128); `rows`: packed rows per tile.
+// paged_tc_few.cu: 16, 32 or 64 rows, one block per SM
+int launch_few(const Args& a, int rows, int blocks, cudaStream_t st);
+
 }  // namespace paged
 }  // namespace pe
