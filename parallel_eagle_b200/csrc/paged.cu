@@ -301,7 +301,7 @@ int launch_simt(int dtype, const Args& a, int blocks, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ kernel choice ----
-enum Kind { kSimt, kFew };
+enum Kind { kSimt, kFew, kMany };
 
 struct Phase {
   Kind kind;
@@ -312,8 +312,8 @@ Phase simt_phase(int hd) { return {kSimt, kSimtRows, sm_count() * (hd <= 128 ? 4
 
 // tensor-core kernel for `rows` packed rows (on average) per request and KV head
 Phase tc_phase(int64_t rows) {
-  const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  return {kFew, n, sm_count()};
+  if (rows > 64) return {kMany, 256, sm_count()};
+  return {kFew, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, sm_count()};
 }
 
 bool tc_sizes(int dtype, int hd) { return dtype == PE_BF16 && (hd == 64 || hd == 128); }
@@ -342,8 +342,9 @@ void carve(Args& a, const Phase& p, uint8_t* ws) {
 }
 
 int run_phase(int dtype, const Phase& p, const Args& a, cudaStream_t st) {
-  const int rc = p.kind == kFew ? launch_few(a, p.Mt, p.blocks, st)
-                                : launch_simt(dtype, a, p.blocks, st);
+  const int rc = p.kind == kFew    ? launch_few(a, p.Mt, p.blocks, st)
+                 : p.kind == kMany ? launch_many(a, p.blocks, st)
+                                   : launch_simt(dtype, a, p.blocks, st);
   if (rc) return rc;
   return launch_join(dtype, a, p.blocks, p.Mt, st);
 }

@@ -67,6 +67,20 @@ struct Req {
   int64_t A;          // cost model: (A + slope terms), see cost()
 };
 
+// A segment as the tensor-core kernels' warps hand it round in shared memory: one warp
+// walks the line of work, the others read.
+struct Seg {
+  int64_t kend;    // keys the tile's last row sees (exclusive end)
+  int64_t lim0;    // keys the tile's first row sees
+  const int32_t* pages;
+  int row0;        // first row of the request
+  int r0, rows;    // first packed row of the tile, packed rows in it
+  int kvh;
+  int t0, t1;      // key tiles
+  int slot;        // of the partial result; -1: the segment is its whole entity
+  int end;         // 1: no more segments
+};
+
 template <int Mt, int TK>
 struct Sched {
   const Args& a;
@@ -214,6 +228,19 @@ struct Sched {
   __device__ __forceinline__ const int32_t* pages() const {
     return a.table + (a.all_rows ? 0 : (int64_t)b * a.table_ld);
   }
+  __device__ __forceinline__ void describe(Seg& g) const {
+    g.kend = kend;
+    g.lim0 = limit(rt * Mt);
+    g.pages = pages();
+    g.row0 = rq.row0;
+    g.r0 = rt * Mt;
+    g.rows = tile_rows();
+    g.kvh = kvh;
+    g.t0 = t0;
+    g.t1 = t1;
+    g.slot = whole() ? -1 : slot();
+    g.end = 0;
+  }
   // recorded by one thread for a segment that is its entity's first piece but not all of it
   __device__ __forceinline__ void record_open() const {
     Open r{};
@@ -263,6 +290,8 @@ __device__ __forceinline__ RowScale finish_row(const Args& a, int t, int head, f
 // Tensor-core kernels (bf16, head sizes 64 and 128); `rows`: packed rows per tile.
 // paged_tc_few.cu: 16, 32 or 64 rows, one block per SM
 int launch_few(const Args& a, int rows, int blocks, cudaStream_t st);
+// paged_tc_many.cu: 256 rows, one block per SM
+int launch_many(const Args& a, int blocks, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace pe
