@@ -204,82 +204,110 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
 }
 
 // ---------------------------------------------------------------------- join ----
-// Block (c, row): joins the pieces of the entity that starts in block c, one of its rows.
-// Pieces are weighted with 2^(m_i - max m) and added in a fixed order: the warps take
-// pieces in turn, and their sums are added warp by warp.
+// Block (c, y): joins the pieces of the entity that starts in block c, rows 4y .. 4y + 3.
+// Pieces are weighted with 2^(m_i - max m) and added in a fixed order.  A warp joins a row;
+// when an entity lies in many pieces (a few long requests over all SMs) the four warps
+// share each row's pieces instead, as one warp's loads would run one after another.
 constexpr int kJoinThreads = 128;
+constexpr int kJoinRows = 4;
+constexpr int kJoinSplit = 16;  // pieces from which the warps share a row
 
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ Args a, int Mt) {
-  extern __shared__ float sw[];  // [parts] weights, then [warps][hd] sums
+  extern __shared__ float sw[];  // [warps][blocks] weights
+  __shared__ float sums[kJoinRows][256];
   const Open op = a.open[blockIdx.x];
-  const int row = blockIdx.y;
-  if (op.parts == 0 || row >= op.rows) return;
+  const int row_base = blockIdx.y * kJoinRows;
+  if (op.parts == 0 || row_base >= op.rows) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int NW = kJoinThreads / 32;
-  __shared__ float red[NW];
-  auto slot_row = [&](int i) {
-    const int s = i == 0 ? op.slot : 2 * ((int)blockIdx.x + i);
-    return (int64_t)s * Mt + row;
-  };
-  float mx = -INFINITY;
-  for (int i = tid; i < op.parts; i += kJoinThreads)
-    if (a.part_ml[2 * slot_row(i) + 1] != 0.f) mx = fmaxf(mx, a.part_ml[2 * slot_row(i)]);
-  mx = warp_max(mx);
-  if (lane == 0) red[warp] = mx;
-  __syncthreads();
-  mx = red[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) mx = fmaxf(mx, red[i]);
-  __syncthreads();
-  float l = 0.f;
-  for (int i = tid; i < op.parts; i += kJoinThreads) {
-    const float m = a.part_ml[2 * slot_row(i)], li = a.part_ml[2 * slot_row(i) + 1];
-    const float wgt = li == 0.f ? 0.f : exp2f(m - mx);
-    sw[i] = wgt;
-    l += li == 0.f ? 0.f : wgt * li;
-  }
-  l = warp_sum(l);
-  if (lane == 0) red[warp] = l;
-  __syncthreads();
-  l = red[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) l += red[i];
-  float* sums = sw + op.parts;
-  for (int d = lane; d < a.hd; d += 32) {
-    float o = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < op.parts; i += NW) {
-      const float wgt = sw[i];
-      if (wgt != 0.f) o += wgt * a.part_o[slot_row(i) * a.hd + d];
+  constexpr int E = 256 / 32;  // elements per lane, in runs of V
+  const bool share = op.parts > kJoinSplit;
+  float* wgt = sw + warp * gridDim.x;
+
+  for (int k = 0; k < (share ? kJoinRows : 1); ++k) {
+    const int row = row_base + (share ? k : warp);
+    if (row >= op.rows) break;
+    auto slot_row = [&](int i) {
+      const int s = i == 0 ? op.slot : 2 * ((int)blockIdx.x + i);
+      return (int64_t)s * Mt + row;
+    };
+    auto column = [&](int e) { return (e / V) * (32 * V) + lane * V + e % V; };
+    float mx = -INFINITY;
+    for (int i = lane; i < op.parts; i += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot_row(i));
+      if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
     }
-    sums[warp * a.hd + d] = o;
-  }
-  __syncthreads();
-  const int rr = op.r0 + row;
-  const int tok = op.row0 + rr / a.G, head = op.kvh * a.G + rr % a.G;
-  const RowScale f = finish_row(a, tok, head, mx, l);
-  for (int d = tid; d < a.hd; d += kJoinThreads) {
-    float o = sums[d];
+    mx = warp_max(mx);
+    float l = 0.f;
+    for (int i = lane; i < op.parts; i += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot_row(i));
+      const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
+      wgt[i] = w;
+      l += ml.y == 0.f ? 0.f : w * ml.y;
+    }
+    l = warp_sum(l);
+    __syncwarp();
+    float acc[E];
 #pragma unroll
-    for (int i = 1; i < NW; ++i) o += sums[i * a.hd + d];
-    const int64_t at = ((int64_t)tok * a.Hq + head) * a.hd + d;
-    float x = f.own == 0.f ? 0.f : o * f.own;
-    if (f.pre != 0.f) x += f.pre * a.pre_o[at];
-    if (a.o32)
-      a.o32[at] = x;
-    else
-      static_cast<T*>(a.o)[(int64_t)tok * a.o_ld + (int64_t)head * a.hd + d] = from_f<T>(x);
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int i = share ? warp : 0; i < op.parts; i += share ? kJoinRows : 1) {
+      const float w = wgt[i];
+      const float* src = a.part_o + slot_row(i) * a.hd;
+#pragma unroll
+      for (int e = 0; e < E; e += V) {
+        if (column(e) >= a.hd) continue;
+        float v[V];
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src + column(e));
+          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+          v[0] = src[column(e)];
+        }
+        // (a piece without keys left its accumulator unwritten)
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[e + q] += w == 0.f ? 0.f : w * v[q];
+      }
+    }
+    if (share) {
+      if (k > 0) __syncthreads();  // the row before is read
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (column(e) < a.hd) sums[warp][column(e)] = acc[e];
+      __syncthreads();
+      if (warp != 0) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (column(e) < a.hd)
+          acc[e] = (sums[0][column(e)] + sums[1][column(e)]) +
+                   (sums[2][column(e)] + sums[3][column(e)]);
+    }
+    const int rr = op.r0 + row;
+    const int tok = op.row0 + rr / a.G, head = op.kvh * a.G + rr % a.G;
+    const RowScale f = finish_row(a, tok, head, mx, l);
+    const int64_t at = ((int64_t)tok * a.Hq + head) * a.hd;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int d = column(e);
+      if (d >= a.hd) continue;
+      float x = f.own == 0.f ? 0.f : acc[e] * f.own;
+      if (f.pre != 0.f) x += f.pre * a.pre_o[at + d];
+      if (a.o32)
+        a.o32[at + d] = x;
+      else
+        static_cast<T*>(a.o)[(int64_t)tok * a.o_ld + (int64_t)head * a.hd + d] = from_f<T>(x);
+    }
+    if (lane == 0) a.lse[(int64_t)head * a.T + tok] = f.lse;
   }
-  if (tid == 0) a.lse[(int64_t)head * a.T + tok] = f.lse;
 }
 
 int launch_join(int dtype, const Args& a, int blocks, int Mt, cudaStream_t st) {
-  const size_t smem = (size_t)(blocks + (kJoinThreads / 32) * a.hd) * sizeof(float);
-  const dim3 grid((unsigned)blocks, (unsigned)Mt);
+  const size_t smem = (size_t)blocks * (kJoinThreads / 32) * sizeof(float);
+  const dim3 grid((unsigned)blocks, (unsigned)ceil_div(Mt, kJoinRows));
   return PE_DISPATCH(dtype, T, [&]() -> int {
-    paged_join_kernel<T><<<grid, kJoinThreads, smem, st>>>(a, Mt);
+    auto kern = a.hd % 4 == 0 ? paged_join_kernel<T, 4> : paged_join_kernel<T, 1>;
+    kern<<<grid, kJoinThreads, smem, st>>>(a, Mt);
     PE_LAUNCHED();
     return PE_OK;
   });

@@ -59,6 +59,13 @@ struct Open {
 
 constexpr float kLn2f = 0.6931471805599453f;
 
+// a / b for a, b >= 0 (the 64-bit division costs several times the 32-bit one, and small
+// calls spend their time here)
+__device__ __forceinline__ int64_t div_pos(int64_t x, int64_t y) {
+  if (((x | y) >> 32) == 0) return (uint32_t)x / (uint32_t)y;
+  return x / y;
+}
+
 // one request as a launch sees it
 struct Req {
   int row0, n;        // first row in q, new rows
@@ -150,7 +157,7 @@ struct Sched {
     }
     total = sum;
     // an equal share each, but no piece below two key tiles' work
-    per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)3 * TK * a.G);
+    per = max(div_pos(total + gridDim.x - 1, gridDim.x), (int64_t)3 * TK * a.G);
     pos = min(total, (int64_t)blockIdx.x * per);
     end = min(total, pos + per);
     // the thread whose requests hold pos finds the request
@@ -185,7 +192,7 @@ struct Sched {
     }
     const int64_t head_cost = cost_before(rq, rq.R);
     int64_t off = pos - base;
-    kvh = (int)(off / head_cost);
+    kvh = (int)div_pos(off, head_cost);
     off -= kvh * head_cost;
     // last row tile that starts at or before off
     int lo = 0, hi = rq.R;
@@ -203,8 +210,8 @@ struct Sched {
     nt = kend > a.kbeg ? (int)((kend - a.kbeg + TK - 1) / TK) : 0;
     first = u0 == 0;
     last = u1 == c;
-    t0 = first ? 0 : (int)(u0 * nt / c);
-    t1 = last ? nt : (int)(u1 * nt / c);
+    t0 = first ? 0 : (int)div_pos(u0 * nt, c);
+    t1 = last ? nt : (int)div_pos(u1 * nt, c);
     entity_end_ = pos - u0 + c;
     pos += u1 - u0;
     ++seg;
@@ -215,7 +222,7 @@ struct Sched {
   __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (seg == 1 ? 0 : 1); }
   // pieces of the current entity, for the block that holds its first piece but not its last
   __device__ __forceinline__ int parts() const {
-    return (int)((entity_end_ - 1) / per) - (int)blockIdx.x + 1;
+    return (int)div_pos(entity_end_ - 1, per) - (int)blockIdx.x + 1;
   }
   // keys that packed row r (of the whole request) sees, as an exclusive end
   __device__ __forceinline__ int64_t limit(int r) const {
