@@ -565,7 +565,8 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           at[e] = a.o32 ? f_at : o_at;
-          pv[e] = c0 + e < live && fac[c0 + e] != 0.f ? fac[c0 + e] * a.pre_o[f_at] : 0.f;
+          // (loads without branches, so that the chunk's eight are in flight together)
+          pv[e] = a.pre_o ? a.pre_o[c0 + e < live ? f_at : tid] : 0.f;
           f_at += HD;
           o_at += HD;
           if (++rem == a.G) {
@@ -577,8 +578,8 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (c0 + e >= live) continue;
-          const float own = mneg[c0 + e];
-          const float v = (!any || own == 0.f ? 0.f : ov[e] * own) + pv[e];
+          const float own = mneg[c0 + e], pre = fac[c0 + e];
+          const float v = (!any || own == 0.f ? 0.f : ov[e] * own) + (pre == 0.f ? 0.f : pre * pv[e]);
           if (a.o32)
             a.o32[at[e]] = v;
           else

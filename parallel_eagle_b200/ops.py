@@ -8,6 +8,7 @@ allocated here (torch owns all memory); the library itself never allocates.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -452,41 +453,49 @@ def attn_bwd_segments(q, k, v, o, do, lse, n_heads, n_kv_heads, head_dim, bounds
 # ----------------------------------------------------- key/value cache ----
 
 
-def _same_device(*ts: torch.Tensor) -> torch.device:
-    """The device all operands are on, which has to be the current one (a kernel
-    launched for another device's memory would run on the current device's stream)."""
+# (These calls are a few microseconds of device work each: their checks are written to cost
+# little, and say what was wrong only once something was.)
+
+
+def _one_device(*ts: torch.Tensor) -> int:
+    """Index of the device all operands are on, which has to be the current one (a kernel
+    for another device's memory would run on the current device's stream)."""
+    idx = ts[0].get_device()
+    if idx >= 0:
+        for t in ts:
+            if t.get_device() != idx:
+                break
+        else:
+            if idx == torch._C._cuda_getDevice():
+                return idx
+            raise L.PeError(f"operands on cuda:{idx}, but the current device is "
+                            f"cuda:{torch.cuda.current_device()} (use torch.cuda.device)")
     L.require_cuda(*ts)
-    dev = ts[0].device
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise L.PeError(f"operands on {dev} and {t.device}: one device is needed")
-    if dev.index != torch.cuda.current_device():
-        raise L.PeError(f"operands on {dev}, but the current device is "
-                        f"cuda:{torch.cuda.current_device()} (use torch.cuda.device)")
-    return dev
+    raise L.PeError("operands on several devices: " + ", ".join(str(t.device) for t in ts))
 
 
-def _ints(what: str, t: torch.Tensor, n: int | None, dtype: torch.dtype) -> None:
-    if t.dim() != 1 or t.dtype != dtype or not t.is_contiguous() or n not in (None, t.shape[0]):
-        want = "" if n is None else f"[{n}] "
-        raise L.PeError(f"{what} must be a contiguous {want}{dtype} vector, got "
-                        f"{tuple(t.shape)} {t.dtype}")
+def _refuse_ints(what: str, t: torch.Tensor, shape: str, dtype: torch.dtype):
+    raise L.PeError(f"{what} must be a contiguous {dtype} tensor [{shape}], got "
+                    f"{tuple(t.shape)} {t.dtype}")
 
 
-def _block_table(what: str, table: torch.Tensor, batch: int) -> None:
-    if (table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != batch
-            or table.shape[1] < 1 or (table.stride(1) != 1 and table.shape[1] > 1)):
+def _table_stride(what: str, table: torch.Tensor, batch: int) -> int:
+    shape = table.shape
+    if (len(shape) != 2 or shape[0] != batch or table.dtype is not torch.int32 or shape[1] < 1
+            or (table.stride(1) != 1 and shape[1] > 1)):
         raise L.PeError(f"{what}: the block table must be int32 [{batch}, pages] with unit column "
-                        f"stride, got {tuple(table.shape)} {table.dtype}")
+                        f"stride, got {tuple(shape)} {table.dtype}")
+    return table.stride(0) if batch > 1 else max(table.stride(0), shape[1])
 
 
-def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
-    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype
-            or not k_cache.is_contiguous() or not v_cache.is_contiguous() or 0 in k_cache.shape):
+def _caches(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor):
+    shape = k_cache.shape
+    if (len(shape) != 4 or shape != v_cache.shape or k_cache.dtype is not v_cache.dtype
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous() or 0 in shape):
         raise L.PeError(f"{what}: the caches must be two contiguous [pages, kv heads, page, "
-                        f"head_dim] tensors of one dtype, got {tuple(k_cache.shape)} "
-                        f"{k_cache.dtype} and {tuple(v_cache.shape)} {v_cache.dtype}")
-    return tuple(k_cache.shape)
+                        f"head_dim] tensors of one dtype, got {tuple(shape)} {k_cache.dtype} "
+                        f"and {tuple(v_cache.shape)} {v_cache.dtype}")
+    return shape
 
 
 def cache_plan(lens, new_lens, table, free, ring, page: int, rows: int, *, shared: int = 0,
@@ -505,48 +514,56 @@ def cache_plan(lens, new_lens, table, free, ring, page: int, rows: int, *, share
     belong to a shared prefix and are left alone."""
     if ring_out is None:
         ring_out = torch.empty_like(ring)
-    dev = _same_device(lens, new_lens, table, free, ring, ring_out)
-    batch = lens.shape[0] if lens.dim() == 1 else -1
-    _ints("cache_plan: lens", lens, batch, torch.int32)
-    _ints("cache_plan: new_lens", new_lens, batch, torch.int32)
-    _ints("cache_plan: free", free, None, torch.int32)
-    _ints("cache_plan: ring", ring, 3, torch.int64)
-    _ints("cache_plan: ring_out", ring_out, 3, torch.int64)
-    _block_table("cache_plan", table, batch)
-    # slots and pos, then granted and cu, from one allocation each
-    rows = int(rows)
+    idx = _one_device(lens, new_lens, table, free, ring, ring_out)
+    batch = lens.numel()
+    for what, t in (("lens", lens), ("new_lens", new_lens)):
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != batch or not t.is_contiguous():
+            _refuse_ints("cache_plan: " + what, t, str(batch), torch.int32)
+    if free.dtype is not torch.int32 or free.dim() != 1 or not free.is_contiguous():
+        _refuse_ints("cache_plan: free", free, "pages", torch.int32)
+    for t in (ring, ring_out):
+        if t.dtype is not torch.int64 or t.dim() != 1 or t.numel() != 3 or not t.is_contiguous():
+            _refuse_ints("cache_plan: ring and ring_out", t, "3", torch.int64)
+    table_ld = _table_stride("cache_plan", table, batch)
     if rows < 0:
         raise L.PeError(f"cache_plan: {rows} new rows")
-    per_row = torch.empty(2, rows, dtype=torch.int64, device=dev)
-    per_req = torch.empty(2 * batch + 1, dtype=torch.int32, device=dev)
-    granted, cu = per_req[:batch], per_req[batch:]
+    dev = lens.device
+    granted = torch.empty_like(lens)
+    cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    pos = torch.empty_like(slots)
     rc = _lib().pe_cache_plan(
-        batch, table.shape[1], free.shape[0], int(page), rows, int(shared), lens.data_ptr(),
-        new_lens.data_ptr(), table.data_ptr(), _row_stride(table), free.data_ptr(),
-        ring.data_ptr(), ring_out.data_ptr(), granted.data_ptr(), cu.data_ptr(),
-        per_row.data_ptr(), per_row.data_ptr() + 8 * rows, L.stream_ptr(dev),
+        batch, table.shape[1], free.numel(), page, rows, shared, lens.data_ptr(),
+        new_lens.data_ptr(), table.data_ptr(), table_ld, free.data_ptr(), ring.data_ptr(),
+        ring_out.data_ptr(), granted.data_ptr(), cu.data_ptr(), slots.data_ptr(), pos.data_ptr(),
+        torch._C._cuda_getCurrentRawStream(idx),
     )
-    L.check(rc, "pe_cache_plan")
-    return granted, cu, per_row[0], per_row[1], ring_out
+    if rc:
+        L.check(rc, "pe_cache_plan")
+    return granted, cu, slots, pos, ring_out
 
 
 def cache_append(k, v, slots, k_cache, v_cache) -> None:
     """Write row t of ``k`` and ``v`` (``[rows, kv heads * head_dim]`` row views, keys already
     rotated) into slot ``slots[t]`` (int64) of the caches; rows whose slot lies outside the
     cache (-1) are skipped.  Slots of one call are distinct, as :func:`cache_plan` gives them."""
-    dev = _same_device(k, v, slots, k_cache, v_cache)
+    idx = _one_device(k, v, slots, k_cache, v_cache)
     pages, hkv, page, hd = _caches("cache_append", k_cache, v_cache)
-    if (k.dim() != 2 or k.shape != v.shape or k.shape[1] != hkv * hd
-            or k.dtype != k_cache.dtype or v.dtype != k_cache.dtype):
-        raise L.PeError(f"cache_append: k and v must be {k_cache.dtype} [rows, {hkv * hd}], got "
-                        f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    _ints("cache_append: slots", slots, k.shape[0], torch.int64)
+    dtype = k_cache.dtype
+    shape = k.shape
+    if (len(shape) != 2 or shape != v.shape or shape[1] != hkv * hd or k.dtype is not dtype
+            or v.dtype is not dtype):
+        raise L.PeError(f"cache_append: k and v must be {dtype} [rows, {hkv * hd}], got "
+                        f"{tuple(shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    if slots.dtype is not torch.int64 or slots.shape != shape[:1] or not slots.is_contiguous():
+        _refuse_ints("cache_append: slots", slots, str(shape[0]), torch.int64)
     rc = _lib().pe_cache_append(
-        L.dtype_code(k.dtype), k.shape[0], hkv, hd, k.data_ptr(), _row_stride(k), v.data_ptr(),
+        L.dtype_code(dtype), shape[0], hkv, hd, k.data_ptr(), _row_stride(k), v.data_ptr(),
         _row_stride(v), slots.data_ptr(), pages, page, k_cache.data_ptr(), v_cache.data_ptr(),
-        L.stream_ptr(dev),
+        torch._C._cuda_getCurrentRawStream(idx),
     )
-    L.check(rc, "pe_cache_append")
+    if rc:
+        L.check(rc, "pe_cache_append")
 
 
 def attn_paged(q, k_cache, v_cache, table, lens, cu, o=None, lse=None, algo=L.ALGO_AUTO):
@@ -567,43 +584,55 @@ def attn_paged_shared(q, k_cache, v_cache, table, lens, cu, shared: int, o=None,
     pages -- samples or drafts forked from one prompt.  The prefix is taken from ``table[0]``
     and read once for all rows; ``lens`` counts it.  Every request with rows holds the whole
     prefix (``lens[b] - n_b >= shared``)."""
-    if int(shared) < 0:
+    if shared < 0:
         raise L.PeError(f"attn_paged_shared: {shared} shared keys")
-    return _attn_paged(q, k_cache, v_cache, table, lens, cu, int(shared), o, lse, algo)
+    return _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_paged_bytes(*sizes: int) -> int:
+    return int(_lib().pe_attn_paged_workspace(*sizes))
 
 
 def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
-    dev = _same_device(q, k_cache, v_cache, table, lens, cu, o, lse)
+    idx = _one_device(q, k_cache, v_cache, table, lens, cu)
     pages, hkv, page, hd = _caches("attn_paged", k_cache, v_cache)
-    if q.dim() != 2 or q.dtype != k_cache.dtype or q.shape[1] % (hkv * hd) or q.shape[1] == 0:
+    dtype = q.dtype
+    if q.dim() != 2 or dtype is not k_cache.dtype or q.shape[1] % (hkv * hd) or q.shape[1] == 0:
         raise L.PeError(f"attn_paged: q must be {k_cache.dtype} [rows, heads * {hd}] with heads a "
-                        f"multiple of {hkv}, got {tuple(q.shape)} {q.dtype}")
-    batch = lens.shape[0] if lens.dim() == 1 else -1
-    _ints("attn_paged: lens", lens, batch, torch.int32)
-    _ints("attn_paged: cu", cu, batch + 1, torch.int32)
-    _block_table("attn_paged", table, batch)
-    T, heads = q.shape[0], q.shape[1] // hd
+                        f"multiple of {hkv}, got {tuple(q.shape)} {dtype}")
+    T, cols = q.shape
+    heads, batch = cols // hd, lens.numel()
+    if lens.dtype is not torch.int32 or lens.dim() != 1 or not lens.is_contiguous():
+        _refuse_ints("attn_paged: lens", lens, "requests", torch.int32)
+    if (cu.dtype is not torch.int32 or cu.dim() != 1 or cu.numel() != batch + 1
+            or not cu.is_contiguous()):
+        _refuse_ints("attn_paged: cu", cu, str(batch + 1), torch.int32)
+    table_ld = _table_stride("attn_paged", table, batch)
+    dev = q.device
     if o is None:
-        o = torch.empty(T, heads * hd, dtype=q.dtype, device=dev)
-    elif o.shape != q.shape or o.dtype != q.dtype:
+        o = torch.empty(T, cols, dtype=dtype, device=dev)
+    elif o.shape != q.shape or o.dtype is not dtype or o.device != dev:
         raise L.PeError(f"attn_paged: o must be like q, got {tuple(o.shape)} {o.dtype}")
     if lse is None:
         lse = torch.empty(heads, T, dtype=torch.float32, device=dev)
-    elif lse.shape != (heads, T) or lse.dtype != torch.float32 or not lse.is_contiguous():
+    elif (lse.shape != (heads, T) or lse.dtype is not torch.float32 or not lse.is_contiguous()
+          or lse.device != dev):
         raise L.PeError(f"attn_paged: lse must be contiguous float32 [{heads}, {T}]")
-    lib = _lib()
-    code = L.dtype_code(q.dtype)
-    nbytes = int(lib.pe_attn_paged_workspace(code, batch, T, heads, hkv, hd, shared))
+    code = L.dtype_code(dtype)
+    nbytes = _attn_paged_bytes(code, batch, T, heads, hkv, hd, shared)
     # the call's own scratch, from torch's stream-ordered allocator: calls on other streams
     # and captured graphs never share it
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    rc = lib.pe_attn_paged(
+    rc = _lib().pe_attn_paged(
         code, batch, T, heads, hkv, hd, q.data_ptr(), _row_stride(q), k_cache.data_ptr(),
-        v_cache.data_ptr(), pages, page, table.data_ptr(), _row_stride(table), table.shape[1],
+        v_cache.data_ptr(), pages, page, table.data_ptr(), table_ld, table.shape[1],
         lens.data_ptr(), cu.data_ptr(), shared, o.data_ptr(), _row_stride(o), lse.data_ptr(),
-        ws.data_ptr(), nbytes, algo, status_word(dev).data_ptr(), L.stream_ptr(dev),
+        ws.data_ptr(), nbytes, algo, status_word(dev).data_ptr(),
+        torch._C._cuda_getCurrentRawStream(idx),
     )
-    L.check(rc, "pe_attn_paged")
+    if rc:
+        L.check(rc, "pe_attn_paged")
     return o, lse
 
 
