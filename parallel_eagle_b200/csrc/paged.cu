@@ -39,7 +39,9 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
   const T* kc = static_cast<const T*>(a.kc);
   const T* vc = static_cast<const T*>(a.vc);
   const int groups = hdp >> 2;  // float4 columns of the output
+  bool joined = false;
 
+  start_next_kernel();
   Sched<Mt, kTK> w(a);
   w.init(scratch);
   if (tid == 0) a.open[blockIdx.x].parts = 0;
@@ -157,6 +159,10 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
       }
       __syncthreads();
     }
+    if (a.pre_lse && !joined) {
+      wait_kernel_before();  // the prefix's rows
+      joined = true;
+    }
     if (w.whole()) {
       if (valid) {
         const int tok = w.rq.row0 + rr / a.G, head = w.kvh * a.G + rr % a.G;
@@ -201,6 +207,7 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
       }
     }
   }
+  wait_kernel_before();  // (also where nothing was joined: the kernels end in order)
 }
 
 // ---------------------------------------------------------------------- join ----
@@ -217,6 +224,8 @@ __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ Args a, int Mt) {
   extern __shared__ float sw[];  // [warps][blocks] weights
   __shared__ float sums[kJoinRows][256];
+  start_next_kernel();
+  wait_kernel_before();
   const Open op = a.open[blockIdx.x];
   const int row_base = blockIdx.y * kJoinRows;
   if (op.parts == 0 || row_base >= op.rows) return;
@@ -307,13 +316,11 @@ int launch_join(int dtype, const Args& a, int blocks, int Mt, cudaStream_t st) {
   const dim3 grid((unsigned)blocks, (unsigned)ceil_div(Mt, kJoinRows));
   return PE_DISPATCH(dtype, T, [&]() -> int {
     auto kern = a.hd % 4 == 0 ? paged_join_kernel<T, 4> : paged_join_kernel<T, 1>;
-    kern<<<grid, kJoinThreads, smem, st>>>(a, Mt);
-    PE_LAUNCHED();
-    return PE_OK;
+    return launch_kernel(kern, grid, kJoinThreads, smem, st, true, a, Mt);
   });
 }
 
-int launch_simt(int dtype, const Args& a, int blocks, cudaStream_t st) {
+int launch_simt(int dtype, const Args& a, int blocks, bool dependent, cudaStream_t st) {
   const int hdp = (a.hd + 3) / 4 * 4;
   const size_t smem = (size_t)((kSimtRows + 2 * kTK) * (hdp + 4) + kSimtRows * kTK) * sizeof(float);
   const int es = dtype == PE_F32 ? 4 : 2;
@@ -322,9 +329,7 @@ int launch_simt(int dtype, const Args& a, int blocks, cudaStream_t st) {
   return PE_DISPATCH(dtype, T, [&]() -> int {
     auto kern = paged_simt_kernel<T>;
     PE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<blocks, kThreads, smem, st>>>(a, hdp, vec);
-    PE_LAUNCHED();
-    return PE_OK;
+    return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, a, hdp, vec);
   });
 }
 
@@ -369,10 +374,10 @@ void carve(Args& a, const Phase& p, uint8_t* ws) {
   a.open = reinterpret_cast<Open*>(ws);
 }
 
-int run_phase(int dtype, const Phase& p, const Args& a, cudaStream_t st) {
-  const int rc = p.kind == kFew    ? launch_few(a, p.Mt, p.blocks, st)
-                 : p.kind == kMany ? launch_many(a, p.blocks, st)
-                                   : launch_simt(dtype, a, p.blocks, st);
+int run_phase(int dtype, const Phase& p, const Args& a, bool dependent, cudaStream_t st) {
+  const int rc = p.kind == kFew    ? launch_few(a, p.Mt, p.blocks, dependent, st)
+                 : p.kind == kMany ? launch_many(a, p.blocks, dependent, st)
+                                   : launch_simt(dtype, a, p.blocks, dependent, st);
   if (rc) return rc;
   return launch_join(dtype, a, p.blocks, p.Mt, st);
 }
@@ -391,8 +396,9 @@ extern "C" size_t pe_attn_paged_workspace(int dtype, int64_t B, int64_t T, int H
   int64_t bytes = phase_bytes(simt_phase(hd), hd);  // (operands may rule the tensor cores out)
   if (tc_sizes(dtype, hd)) bytes = std::max(bytes, phase_bytes(tc_phase(ceil_div(T * G, B)), hd));
   if (shared <= 0) return (size_t)bytes;
-  if (tc_sizes(dtype, hd)) bytes = std::max(bytes, phase_bytes(tc_phase(T * G), hd));
-  return (size_t)(al256(T * Hq * hd * 4) + al256(T * Hq * 4) + bytes);
+  int64_t prefix = phase_bytes(simt_phase(hd), hd);
+  if (tc_sizes(dtype, hd)) prefix = std::max(prefix, phase_bytes(tc_phase(T * G), hd));
+  return (size_t)(al256(T * Hq * hd * 4) + al256(T * Hq * 4) + prefix + bytes);
 }
 
 extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd,
@@ -460,7 +466,8 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     pa.o32 = pre_o;
     pa.lse = pre_lse;
     carve(pa, p, ws);
-    const int rc = run_phase(dtype, p, pa, st);
+    ws += phase_bytes(p, hd);
+    const int rc = run_phase(dtype, p, pa, false, st);
     if (rc) return rc;
     a.kbeg = shared;
     a.pre_o = pre_o;
@@ -468,5 +475,5 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
   }
   const Phase p = tc ? tc_phase(ceil_div(T * a.G, B)) : simt_phase(hd);
   carve(a, p, ws);
-  return run_phase(dtype, p, a, st);
+  return run_phase(dtype, p, a, shared > 0, st);
 }

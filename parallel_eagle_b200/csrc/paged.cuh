@@ -264,6 +264,35 @@ struct Sched {
   int64_t entity_end_;
 };
 
+// The kernels of one call (prefix, its join, the requests' own keys, their join) are launched
+// as programmatic dependents: each may start while the one before it runs, and waits at
+// the point where it reads that one's results.  They share no scratch.
+__device__ __forceinline__ void start_next_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_kernel_before() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// launch, optionally as a dependent of the kernel before it in the stream
+template <typename... P, typename... A>
+inline int launch_kernel(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem,
+                         cudaStream_t st, bool dependent, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = dependent ? 1 : 0;
+  PE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, P(args)...));
+  ++launch_counter();
+  return PE_OK;
+}
+
 // What a finished row's accumulator is multiplied by: o = own * acc + pre * pre_o.
 struct RowScale {
   float own, pre, lse;
@@ -296,9 +325,9 @@ __device__ __forceinline__ RowScale finish_row(const Args& a, int t, int head, f
 
 // Tensor-core kernels (bf16, head sizes 64 and 128); `rows`: packed rows per tile.
 // paged_tc_few.cu: 16, 32 or 64 rows, one block per SM
-int launch_few(const Args& a, int rows, int blocks, cudaStream_t st);
+int launch_few(const Args& a, int rows, int blocks, bool dependent, cudaStream_t st);
 // paged_tc_many.cu: 256 rows, one block per SM
-int launch_many(const Args& a, int blocks, cudaStream_t st);
+int launch_many(const Args& a, int blocks, bool dependent, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace pe

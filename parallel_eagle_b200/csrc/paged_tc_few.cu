@@ -153,6 +153,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* status = a.status;
 
+  start_next_kernel();
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&sm.k_full[i], 1);
@@ -371,7 +372,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     float* fac = sm.fac + cb;
     // A wait that runs out only marks its thread: the group leaves together, at the next
     // barrier that all of its threads reach.
-    bool bad = false;
+    bool bad = false, joined = false;
     int i = 0, seq = 0;
     Seg g;
     for (int s = 0;; ++s) {
@@ -517,6 +518,10 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         if (!(lane & 1)) sm.mx[quarter][cb + (lane >> 1)] = l[0];
       }
       if (vote_group(bar, bad)) break;
+      if (a.pre_lse && !joined) {
+        wait_kernel_before();  // the prefix's rows
+        joined = true;
+      }
       if (tid < live) {
         const int c = cb + tid;
         const float sum = (sm.mx[0][c] + sm.mx[1][c]) + (sm.mx[2][c] + sm.mx[3][c]);
@@ -596,6 +601,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     }
   }
 
+  wait_kernel_before();  // (also where nothing was joined: the kernels end in order)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -605,7 +611,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 }
 
 template <int N, int HDC>
-int launch(const Args& a, int blocks, cudaStream_t st) {
+int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
   int box = kTile;
   while (a.page % box) box >>= 1;  // (pages are multiples of 16)
   CUtensorMap tk, tv;
@@ -616,19 +622,18 @@ int launch(const Args& a, int blocks, cudaStream_t st) {
   auto kern = paged_few_kernel<N, HDC>;
   constexpr int smem = (int)Few<N, HDC>::kSmem;
   PE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  kern<<<blocks, Few<N, HDC>::kThreads, smem, st>>>(tk, tv, a, box);
-  PE_LAUNCHED();
-  return PE_OK;
+  return launch_kernel(kern, dim3((unsigned)blocks), Few<N, HDC>::kThreads, smem, st, dependent, tk,
+                       tv, a, box);
 }
 
 }  // namespace
 
-int launch_few(const Args& a, int rows, int blocks, cudaStream_t st) {
+int launch_few(const Args& a, int rows, int blocks, bool dependent, cudaStream_t st) {
   const bool wide = a.hd == 128;
   switch (rows) {
-    case 16: return wide ? launch<16, 2>(a, blocks, st) : launch<16, 1>(a, blocks, st);
-    case 32: return wide ? launch<32, 2>(a, blocks, st) : launch<32, 1>(a, blocks, st);
-    default: return wide ? launch<64, 2>(a, blocks, st) : launch<64, 1>(a, blocks, st);
+    case 16: return wide ? launch<16, 2>(a, blocks, dependent, st) : launch<16, 1>(a, blocks, dependent, st);
+    case 32: return wide ? launch<32, 2>(a, blocks, dependent, st) : launch<32, 1>(a, blocks, dependent, st);
+    default: return wide ? launch<64, 2>(a, blocks, dependent, st) : launch<64, 1>(a, blocks, dependent, st);
   }
 }
 

@@ -74,6 +74,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* status = a.status;
 
+  start_next_kernel();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.seg_full[i], 1);
@@ -165,21 +166,24 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // ---------------------------------------------------------------- MMA ----
       constexpr uint32_t ID_S = idesc_bf16(kTile, kTile, false, false);
       constexpr uint32_t ID_O = idesc_bf16(kTile, HD, false, true);
+      const uint32_t q_lo = sw128_lo(smem_u32(sQ), 16);
+      const uint32_t kv_lo = sw128_lo(smem_u32(sKV), 16);
+      const uint32_t v_lo = sw128_lo(smem_u32(sKV) + kTileBytes, kChunk);
       auto issue_s = [&](int h, int st) {
-        const uint32_t qa = smem_u32(sQ + h * kTileBytes), kb = smem_u32(sKV + st * 2 * kTileBytes);
+        const uint32_t qa = q_lo + h * (kTileBytes >> 4), kb = kv_lo + st * (2 * kTileBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kChunk + (kk & 3) * 32;
-          mma_bf16_ss(tmem + 256 + h * 128, sw128_desc(qa + off, 16, 1024),
-                      sw128_desc(kb + off, 16, 1024), ID_S, kk > 0 ? 1u : 0u);
+          const uint32_t off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
+          mma_bf16_ss_lo(tmem + 256 + h * 128, qa + off, kb + off, ID_S, kk > 0 ? 1u : 0u);
         }
       };
       auto issue_pv = [&](int h, int st, bool first) {
-        const uint32_t vb = smem_u32(sKV + st * 2 * kTileBytes + kTileBytes);
+        const uint32_t vb = v_lo + st * (2 * kTileBytes >> 4);
+        const uint32_t p = tmem + 256 + h * 128;
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_bf16_ts(tmem + h * 128, tmem + 256 + h * 128 + kk * 8,
-                      sw128_desc(vb + kk * 2048, kChunk, 1024), ID_O, (!first || kk > 0) ? 1u : 0u);
+          mma_bf16_ts_lo(tmem + h * 128, p + kk * 8, vb + kk * (2048 >> 4), ID_O,
+                         kk > 0 ? 1u : first ? 0u : 1u);
       };
       bool ok = true;
       int i = 0, seq = 0;
@@ -300,7 +304,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + 256 + h * 128 + lane_off, tO = tmem + h * 128 + lane_off;
     const float scale = a.scale_log2;
-    bool ok = true;
+    bool ok = true, joined = false;
     int i = 0, seq = 0;
     Seg g;
     for (int s = 0; ok; ++s) {
@@ -408,6 +412,10 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!ok) break;
         tc_fence_after();
       }
+      if (a.pre_lse && !joined) {
+        wait_kernel_before();  // the prefix's rows
+        joined = true;
+      }
       const int orow = g.row0 + tok, head = g.kvh * a.G + rr - tok * a.G;
       RowScale f{0.f, 0.f, 0.f};
       float* po = nullptr;
@@ -481,6 +489,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
   }
 
+  wait_kernel_before();  // (also where nothing was joined: the kernels end in order)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -490,7 +499,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 }
 
 template <int HDC>
-int launch(const Args& a, int blocks, cudaStream_t st) {
+int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
   int box = kTile;
   while (a.page % box) box >>= 1;  // (pages are multiples of 16)
   CUtensorMap tk, tv;
@@ -511,15 +520,14 @@ int launch(const Args& a, int blocks, cudaStream_t st) {
                  "attn_paged: kernel compiled with too few registers");
   }
   const int o_vec = (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 && a.o_ld % 8 == 0;
-  kern<<<blocks, kThreads, smem, st>>>(tk, tv, a, box, o_vec);
-  PE_LAUNCHED();
-  return PE_OK;
+  return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, tk, tv, a, box,
+                       o_vec);
 }
 
 }  // namespace
 
-int launch_many(const Args& a, int blocks, cudaStream_t st) {
-  return a.hd == 128 ? launch<2>(a, blocks, st) : launch<1>(a, blocks, st);
+int launch_many(const Args& a, int blocks, bool dependent, cudaStream_t st) {
+  return a.hd == 128 ? launch<2>(a, blocks, dependent, st) : launch<1>(a, blocks, dependent, st);
 }
 
 }  // namespace paged
