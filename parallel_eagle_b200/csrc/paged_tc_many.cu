@@ -7,16 +7,19 @@
 // heads of a KV head's group) as two 128-row tiles A and B, so the tensor core always has
 // one tile's products to run while the other tile's softmax executes:
 //
-//   warp 0       TMA: K and V tiles of 128 keys, boxes of one page's keys, two stages
-//   warp 1       tcgen05.mma, per key tile:  PV_A(j) S_A(j+1) PV_B(j) S_B(j+1)
+//   warp 0       TMA: K and V tiles of 64 keys, boxes of one page's keys, through two rings
+//   warp 1       tcgen05.mma, per key tile:  PV_A(j) S_A(j+2) PV_B(j) S_B(j+2)
 //                (S = Q K^T into TMEM; P read from TMEM as the A operand)
 //   warp 2       walks the line of work and publishes segments; warps 2..3 fetch Q rows
 //   warps 4..7   softmax of tile A, one thread per row (TMEM lane); warps 8..11 of tile B
 //
-// TMEM: O_A columns 0..127, O_B 128..255, S_A 256..383, S_B 384..511; P overwrites the first
-// 64 columns of its S as packed bf16 pairs.  A row's maximum is only raised (and O rescaled)
-// when it grows by more than 2^8.  Every fourth pair of exponentials runs on the FMA pipe,
-// as the SFU's 16 per clock would take longer than the products.
+// TMEM: O_A columns 0..127, O_B 128..255, two S of 64 columns for A and two for B behind
+// them; P overwrites the first 32 columns of its S as packed bf16 pairs.  With two S a tile
+// the next scores are there when a softmax ends, so both tiles' softmax run all the time;
+// with one S of 128 keys they took turns with their own products (3840 cycles per 128
+// keys, the tensor pipe half idle).  A row's maximum is only raised (and O rescaled) when
+// it grows by more than 2^8.  Every fourth pair of exponentials runs on the FMA pipe, as
+// the SFU's 16 per clock would take longer than the products.
 #include "paged.cuh"
 #include "sm100.cuh"
 
@@ -28,23 +31,27 @@ using namespace sm100;
 
 constexpr int kThreads = 384;
 constexpr int kRows = 256;                    // packed rows per block
-constexpr int kTile = 128;                    // keys per tile, rows per softmax group
-constexpr uint32_t kChunk = kTile * 128;      // 128 rows x 64 columns, 128-byte swizzled
-constexpr int kRegsLow = 88, kRegsHigh = 208; // 128 x 88 + 256 x 208 = 384 x 168
+constexpr int kHalf = 128;                    // rows per softmax group
+constexpr int kTile = 64;                     // keys per tile
+constexpr int kStages = 4;                    // K tiles, V tiles in shared memory
+constexpr uint32_t kChunk = kTile * 128;      // 64 keys x 64 columns, 128-byte swizzled
+constexpr uint32_t kQChunk = kHalf * 128;     // 128 rows x 64 columns
 constexpr float kRaise = 8.f;
 constexpr int kEmuEvery = 4;
 
 struct Small {
   Seg seg[2];
   int64_t scratch[kThreads / 32 + 4];
-  uint64_t seg_full[2], seg_empty[2], kv_full[2], kv_empty[2];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t seg_full[2], seg_empty[2];
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t q_full, q_empty, o_full[2], o_empty[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2];  // [row tile] ([S buffer])
   uint32_t tmem;
 };
 
 template <int HDC>
 constexpr size_t smem_bytes() {
-  return 1024 + 6 * HDC * kChunk /* Q_A, Q_B, two stages of K and V */ + sizeof(Small);
+  return 1024 + 2 * HDC * kQChunk /* Q_A, Q_B */ + 2 * kStages * HDC * kChunk + sizeof(Small);
 }
 
 __device__ __forceinline__ uint32_t swz128(int r, int u) {
@@ -64,13 +71,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ Args a, int box, int o_vec) {
   constexpr int HD = 64 * HDC;
-  constexpr uint32_t kTileBytes = HDC * kChunk;
+  constexpr uint32_t kTileBytes = HDC * kChunk, kQBytes = HDC * kQChunk;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* sQ = smem;                    // tile t at + t * kTileBytes
-  uint8_t* sKV = sQ + 2 * kTileBytes;    // stage s: K at + s * 2 * kTileBytes, V behind it
-  Small& sm = *reinterpret_cast<Small*>(sKV + 4 * kTileBytes);
+  uint8_t* sQ = smem;  // row tile h at + h * kQBytes
+  uint8_t* sK = sQ + 2 * kQBytes;
+  uint8_t* sV = sK + kStages * kTileBytes;
+  Small& sm = *reinterpret_cast<Small*>(sV + kStages * kTileBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* status = a.status;
 
@@ -78,13 +86,20 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.seg_full[i], 1);
-      mbar_init(&sm.seg_empty[i], 12);  // every warp reads it
-      mbar_init(&sm.kv_full[i], 1);
-      mbar_init(&sm.kv_empty[i], 1);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], 4);
+      mbar_init(&sm.seg_empty[i], kThreads / 32);  // every warp reads it
       mbar_init(&sm.o_full[i], 1);
       mbar_init(&sm.o_empty[i], 4);
+      mbar_init(&sm.pv_done[i], 1);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&sm.s_full[i][j], 1);
+        mbar_init(&sm.p_full[i][j], 4);
+      }
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
     }
     mbar_init(&sm.q_full, 2);
     mbar_init(&sm.q_empty, 1);
@@ -116,12 +131,11 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   };
   // keys that tile A's last row sees
   auto kend_a = [&](const Seg& g) -> int64_t {
-    if (a.all_rows || g.rows <= kTile) return g.kend;
-    return min(g.kend, g.lim0 + (g.r0 + kTile - 1) / a.G - g.r0 / a.G);
+    if (a.all_rows || g.rows <= kHalf) return g.kend;
+    return min(g.kend, g.lim0 + (g.r0 + kHalf - 1) / a.G - g.r0 / a.G);
   };
 
   if (warp < 4) {
-    setmaxnreg_dec<kRegsLow>();
     if (warp == 0) {
       // ---------------------------------------------------------------- TMA ----
       const int per_chunk = kTile / box, boxes = per_chunk * HDC;
@@ -129,6 +143,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int total_rows = (int)(a.num_pages * a.Hkv * a.page);
       bool ok = true;
       int i = 0;
+      uint32_t st = 0, ph = 0;
       Seg g;
       for (int s = 0; ok; ++s) {
         ok = take(s, g);
@@ -139,47 +154,57 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           const bool mine = lane < boxes && at < live;
           int row = total_rows;  // (reads as zeros)
           if (mine) {
-            const int64_t key = k0 + at * box, pi = key / a.page;
+            const int64_t key = k0 + at * box, pi = div_pos(key, a.page);
             const int id = g.pages[pi];
             if (id >= 0 && id < a.num_pages)
               row = (int)(((int64_t)id * a.Hkv + g.kvh) * a.page + (key - pi * a.page));
           }
-          const int st = i & 1;
-          ok = mbar_wait(&sm.kv_empty[st], ((i >> 1) & 1) ^ 1u, status, 422);
+          const uint32_t bytes = (uint32_t)live * HDC * box * 128;
+          const uint32_t off = st * kTileBytes + ch * kChunk + at * box * 128;
+          ok = mbar_wait(&sm.k_empty[st], ph ^ 1u, status, 422);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          uint8_t* dst = sKV + st * 2 * kTileBytes + ch * kChunk + at * box * 128;
-          if (lane == 0)
-            mbar_arrive_expect_tx(&sm.kv_full[st], (uint32_t)live * 2 * HDC * box * 128);
+          if (lane == 0) mbar_arrive_expect_tx(&sm.k_full[st], bytes);
           __syncwarp();
-          if (mine) {
-            tma_load_2d(dst, &tmK, &sm.kv_full[st], ch * 64, row);
-            tma_load_2d(dst + kTileBytes, &tmV, &sm.kv_full[st], ch * 64, row);
+          if (mine) tma_load_2d(sK + off, &tmK, &sm.k_full[st], ch * 64, row);
+          ok = mbar_wait(&sm.v_empty[st], ph ^ 1u, status, 423);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) {
+            mbar_wait(&sm.k_full[st], ph, nullptr, 0);  // its copies land before the block ends
+            break;
           }
+          if (lane == 0) mbar_arrive_expect_tx(&sm.v_full[st], bytes);
+          __syncwarp();
+          if (mine) tma_load_2d(sV + off, &tmV, &sm.v_full[st], ch * 64, row);
+          if (++st == kStages) { st = 0; ph ^= 1u; }
         }
       }
       if (!ok) {  // copies in flight land before the block ends
-        for (int back = 1; back <= 2 && back <= i; ++back)
-          mbar_wait(&sm.kv_full[(i - back) & 1], ((i - back) >> 1) & 1, nullptr, 0);
+        for (int back = 1; back <= kStages && back <= i; ++back) {
+          const int j = i - back;
+          mbar_wait(&sm.k_full[j % kStages], (j / kStages) & 1, nullptr, 0);
+          mbar_wait(&sm.v_full[j % kStages], (j / kStages) & 1, nullptr, 0);
+        }
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA ----
-      constexpr uint32_t ID_S = idesc_bf16(kTile, kTile, false, false);
-      constexpr uint32_t ID_O = idesc_bf16(kTile, HD, false, true);
+      constexpr uint32_t ID_S = idesc_bf16(kHalf, kTile, false, false);
+      constexpr uint32_t ID_O = idesc_bf16(kHalf, HD, false, true);
       const uint32_t q_lo = sw128_lo(smem_u32(sQ), 16);
-      const uint32_t kv_lo = sw128_lo(smem_u32(sKV), 16);
-      const uint32_t v_lo = sw128_lo(smem_u32(sKV) + kTileBytes, kChunk);
-      auto issue_s = [&](int h, int st) {
-        const uint32_t qa = q_lo + h * (kTileBytes >> 4), kb = kv_lo + st * (2 * kTileBytes >> 4);
+      const uint32_t k_lo = sw128_lo(smem_u32(sK), 16);
+      const uint32_t v_lo = sw128_lo(smem_u32(sV), kChunk);
+      auto issue_s = [&](int h, int j) {
+        const uint32_t qa = q_lo + h * (kQBytes >> 4);
+        const uint32_t kb = k_lo + (j % kStages) * (kTileBytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * kChunk + (kk & 3) * 32) >> 4;
-          mma_bf16_ss_lo(tmem + 256 + h * 128, qa + off, kb + off, ID_S, kk > 0 ? 1u : 0u);
-        }
+        for (int kk = 0; kk < HD / 16; ++kk)
+          mma_bf16_ss_lo(tmem + 256 + h * 128 + (j & 1) * 64,
+                         qa + (((kk >> 2) * kQChunk + (kk & 3) * 32) >> 4),
+                         kb + (((kk >> 2) * kChunk + (kk & 3) * 32) >> 4), ID_S, kk > 0 ? 1u : 0u);
       };
-      auto issue_pv = [&](int h, int st, bool first) {
-        const uint32_t vb = v_lo + st * (2 * kTileBytes >> 4);
-        const uint32_t p = tmem + 256 + h * 128;
+      auto issue_pv = [&](int h, int j, bool first) {
+        const uint32_t vb = v_lo + (j % kStages) * (kTileBytes >> 4);
+        const uint32_t p = tmem + 256 + h * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
           mma_bf16_ts_lo(tmem + h * 128, p + kk * 8, vb + kk * (2048 >> 4), ID_O,
@@ -193,52 +218,46 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!ok || g.end) break;
         if (g.t1 <= g.t0) continue;
         const int64_t ka = kend_a(g);
-        const bool two = g.rows > kTile;
+        const bool two = g.rows > kHalf;
+        const int n = g.t1 - g.t0;
+        // tiles of the segment that tile A sees
+        const int na = (int)max((int64_t)0, min((int64_t)n, (ka - a.kbeg + kTile - 1) / kTile - g.t0));
         if (elect_one()) {
-          auto use_a = [&](int t) { return a.kbeg + (int64_t)t * kTile < ka; };
-          ok = mbar_wait(&sm.q_full, seq & 1, status, 423) &&
-               mbar_wait(&sm.kv_full[i & 1], (i >> 1) & 1, status, 424);
-          if (ok) {
-            tc_fence_after();
-            if (use_a(g.t0)) issue_s(0, i & 1);
-            mma_commit(&sm.s_full[0]);
-            if (two) issue_s(1, i & 1);
-            mma_commit(&sm.s_full[1]);
-            if (g.t0 + 1 == g.t1) mma_commit(&sm.q_empty);
-          }
-          bool pv_a = false, pv_b = false;
-          for (int t = g.t0, j = i; t < g.t1 && ok; ++t, ++j) {
-            const int st = j & 1, sn = st ^ 1;
-            const bool more = t + 1 < g.t1;
-            if (!mbar_wait(&sm.p_full[0], j & 1, status, 425)) { ok = false; break; }
-            if (t == g.t0 && (!mbar_wait(&sm.o_empty[0], (seq & 1) ^ 1u, status, 426) ||
-                              !mbar_wait(&sm.o_empty[1], (seq & 1) ^ 1u, status, 427))) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            if (use_a(t)) {
-              issue_pv(0, st, !pv_a);
-              pv_a = true;
-            }
-            if (more) {
-              if (!mbar_wait(&sm.kv_full[sn], ((j + 1) >> 1) & 1, status, 428)) { ok = false; break; }
+          // scores of the segment's tile u into the buffer that tile u - 2 left
+          auto scores = [&](int h, int u) -> bool {
+            const int j = i + u;
+            if (h == 0) {
+              if (!mbar_wait(&sm.k_full[j % kStages], (j / kStages) & 1, status, 425)) return false;
               tc_fence_after();
-              if (use_a(t + 1)) issue_s(0, sn);
-              mma_commit(&sm.s_full[0]);
             }
-            if (!mbar_wait(&sm.p_full[1], j & 1, status, 429)) { ok = false; break; }
+            if (h == 0 ? u < na : two) issue_s(h, j);
+            mma_commit(&sm.s_full[h][j & 1]);
+            if (h == 1) {
+              mma_commit(&sm.k_empty[j % kStages]);
+              if (u + 1 == n) mma_commit(&sm.q_empty);
+            }
+            return true;
+          };
+          ok = mbar_wait(&sm.q_full, seq & 1, status, 424);
+          for (int u = 0; u < 2 && u < n && ok; ++u) ok = scores(0, u) && scores(1, u);
+          for (int u = 0; u < n && ok; ++u) {
+            const int j = i + u;
+            ok = mbar_wait(&sm.v_full[j % kStages], (j / kStages) & 1, status, 426) &&
+                 mbar_wait(&sm.p_full[0][j & 1], (j >> 1) & 1, status, 427) &&
+                 (u > 0 || (mbar_wait(&sm.o_empty[0], (seq & 1) ^ 1u, status, 428) &&
+                            mbar_wait(&sm.o_empty[1], (seq & 1) ^ 1u, status, 429)));
+            if (!ok) break;
             tc_fence_after();
-            if (two) {
-              issue_pv(1, st, !pv_b);
-              pv_b = true;
-            }
-            if (more) {
-              if (two) issue_s(1, sn);
-              mma_commit(&sm.s_full[1]);
-              if (t + 2 == g.t1) mma_commit(&sm.q_empty);
-            }
-            mma_commit(&sm.kv_empty[st]);
+            if (u < na) issue_pv(0, j, u == 0);
+            mma_commit(&sm.pv_done[0]);
+            if (u + 2 < n && !scores(0, u + 2)) { ok = false; break; }
+            ok = mbar_wait(&sm.p_full[1][j & 1], (j >> 1) & 1, status, 430);
+            if (!ok) break;
+            tc_fence_after();
+            if (two) issue_pv(1, j, u == 0);
+            mma_commit(&sm.pv_done[1]);
+            mma_commit(&sm.v_empty[j % kStages]);
+            if (u + 2 < n && !scores(1, u + 2)) { ok = false; break; }
           }
           if (ok) {
             mma_commit(&sm.o_full[0]);
@@ -246,7 +265,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
         }
         ok = __all_sync(0xffffffffu, ok);
-        i += g.t1 - g.t0;
+        i += n;
         ++seq;
       }
     } else {
@@ -257,7 +276,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       Seg g;
       for (int s = 0; ok; ++s) {
         if (warp == 2) {
-          ok = mbar_wait(&sm.seg_empty[s & 1], ((s >> 1) & 1) ^ 1u, status, 430);
+          ok = mbar_wait(&sm.seg_empty[s & 1], ((s >> 1) & 1) ^ 1u, status, 432);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const bool have = w.next();
@@ -275,16 +294,16 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         ok = take(s, g);
         if (!ok || g.end) break;
         if (g.t1 <= g.t0) continue;
-        ok = mbar_wait(&sm.q_empty, (seq & 1) ^ 1u, status, 431);
+        ok = mbar_wait(&sm.q_empty, (seq & 1) ^ 1u, status, 433);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         constexpr int U = HD / 8;
-        const int n = g.rows > kTile ? kRows : kTile;
+        const int n = g.rows > kHalf ? kRows : kHalf;
         for (int x = threadIdx.x - 64; x < n * U; x += 64) {
           const int r = x / U, u = x % U;
           const bool valid = r < g.rows;
           const int pr = g.r0 + (valid ? r : 0), tok = pr / a.G;
-          cp_async16(sQ + (r >> 7) * kTileBytes + (u >> 3) * kChunk + swz128(r & 127, u & 7),
+          cp_async16(sQ + (r >> 7) * kQBytes + (u >> 3) * kQChunk + swz128(r & 127, u & 7),
                      q + (int64_t)(g.row0 + tok) * a.q_ld +
                          (int64_t)(g.kvh * a.G + pr - tok * a.G) * HD + u * 8,
                      valid);
@@ -297,12 +316,11 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
     }
   } else {
-    setmaxnreg_inc<kRegsHigh>();
     // --------------------------------------------------------------- softmax ----
     const int h = (warp - 4) >> 2;  // row tile A or B
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + 256 + h * 128 + lane_off, tO = tmem + h * 128 + lane_off;
+    const uint32_t tO = tmem + h * 128 + lane_off;
     const float scale = a.scale_log2;
     bool ok = true, joined = false;
     int i = 0, seq = 0;
@@ -310,35 +328,36 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     for (int s = 0; ok; ++s) {
       ok = take(s, g);
       if (!ok || g.end) break;
-      const int rr = g.r0 + h * kTile + row;  // packed row of the request
-      const bool valid = h * kTile + row < g.rows;
+      const int rr = g.r0 + h * kHalf + row;  // packed row of the request
+      const bool valid = h * kHalf + row < g.rows;
       const int tok = rr / a.G;
       const int64_t lim = !valid ? -1 : a.all_rows ? g.kend
                           : min(g.kend, g.lim0 + tok - g.r0 / a.G);
       // the group's tiles: those some row of it sees
-      const int64_t gend = h == 0 ? kend_a(g) : g.rows > kTile ? g.kend : -1;
+      const int64_t gend = h == 0 ? kend_a(g) : g.rows > kHalf ? g.kend : -1;
       float m = -INFINITY, l = 0.f;
       for (int t = g.t0; t < g.t1; ++t, ++i) {
-        ok = mbar_wait(&sm.s_full[h], i & 1, status, 432);
+        const uint32_t tS = tmem + 256 + h * 128 + (i & 1) * 64 + lane_off;
+        ok = mbar_wait(&sm.s_full[h][i & 1], (i >> 1) & 1, status, 434);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         const int64_t k0 = a.kbeg + (int64_t)t * kTile;
         if (k0 < gend) {
-          float x[128];
-#pragma unroll
-          for (int c = 0; c < 128; c += 32) tmem_ld32(tS + c, x + c);
+          float x[64];
+          tmem_ld32(tS, x);
+          tmem_ld32(tS + 32, x + 32);
           tmem_wait_ld();
           if (k0 + kTile > lim) {
             const int see = (int)max((int64_t)0, lim - k0);
 #pragma unroll
-            for (int c = 0; c < 128; ++c) x[c] = c < see ? x[c] : -INFINITY;
+            for (int c = 0; c < 64; ++c) x[c] = c < see ? x[c] : -INFINITY;
           }
           float mp[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) mp[u] = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 128; c += 8) {
+          for (int c = 0; c < 64; c += 8) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) mp[u] = max3f(mp[u], x[c + 2 * u], x[c + 2 * u + 1]);
           }
@@ -354,28 +373,29 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
           for (int u = 0; u < 4; ++u) rs[u] = make_float2(0.f, 0.f);
           const float2 sc = make_float2(scale, scale), off = make_float2(nm, nm);
+          uint32_t pk[32];
 #pragma unroll
-          for (int c0 = 0; c0 < 128; c0 += 32) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              const float2 y = fma2(make_float2(x[c0 + c], x[c0 + c + 1]), sc, off);
-              float2 p;
-              if (kEmuEvery > 0 && (c / 2) % kEmuEvery == kEmuEvery - 1) {
-                p = exp2_poly2(y);
-              } else {
-                p.x = ex2_approx(y.x);
-                p.y = ex2_approx(y.y);
-              }
-              rs[(c >> 1) & 3] = add2(rs[(c >> 1) & 3], p);
-              pk[c / 2] = pack_bf16x2(p.x, p.y);
+          for (int c = 0; c < 64; c += 2) {
+            const float2 y = fma2(make_float2(x[c], x[c + 1]), sc, off);
+            float2 p;
+            if (kEmuEvery > 0 && (c / 2) % kEmuEvery == kEmuEvery - 1) {
+              p = exp2_poly2(y);
+            } else {
+              p.x = ex2_approx(y.x);
+              p.y = ex2_approx(y.y);
             }
-            tmem_st16(tS + c0 / 2, pk);
+            rs[(c >> 1) & 3] = add2(rs[(c >> 1) & 3], p);
+            pk[c / 2] = pack_bf16x2(p.x, p.y);
           }
+          tmem_st32(tS, pk);
           const float2 rsum = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
           l += rsum.x + rsum.y;
-          // O holds the tiles before this one (their PV completed before this S did)
+          // O holds the tiles before this one, once their product is done
           if (__any_sync(0xffffffffu, alpha != 1.f) && t > g.t0) {
+            ok = mbar_wait(&sm.pv_done[h], (i - 1) & 1, status, 437);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
               float ov[32];
@@ -388,26 +408,31 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
           }
           tmem_wait_st();
-          if (k0 + kTile > g.kend && k0 + row >= g.kend) {
+          if (k0 + kTile > g.kend) {
             // what lies behind the last key must not meet its zero probabilities (0 x NaN);
-            // both groups write the same zeros
-            uint8_t* v = sKV + (i & 1) * 2 * kTileBytes + kTileBytes;
+            // both row tiles write the same zeros
+            ok = mbar_wait(&sm.v_full[i % kStages], (i / kStages) & 1, status, 435);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (row < kTile && k0 + row >= g.kend) {
+              uint8_t* v = sV + (i % kStages) * kTileBytes;
 #pragma unroll
-            for (int u = 0; u < 8 * HDC; ++u)
-              *reinterpret_cast<uint4*>(v + (u >> 3) * kChunk + swz128(row, u & 7)) =
-                  make_uint4(0, 0, 0, 0);
+              for (int u = 0; u < 8 * HDC; ++u)
+                *reinterpret_cast<uint4*>(v + (u >> 3) * kChunk + swz128(row, u & 7)) =
+                    make_uint4(0, 0, 0, 0);
+            }
           }
           fence_proxy_async();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[h]);
+        if (lane == 0) mbar_arrive(&sm.p_full[h][i & 1]);
       }
       if (!ok) break;
       // ---- the segment's rows ----
       const bool any = g.t1 > g.t0;
       if (any) {
-        ok = mbar_wait(&sm.o_full[h], seq & 1, status, 433);
+        ok = mbar_wait(&sm.o_full[h], seq & 1, status, 436);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -420,7 +445,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       RowScale f{0.f, 0.f, 0.f};
       float* po = nullptr;
       if (g.slot >= 0) {
-        const int64_t prow = (int64_t)g.slot * kRows + h * kTile + row;
+        const int64_t prow = (int64_t)g.slot * kRows + h * kHalf + row;
         po = a.part_o + prow * HD;
         if (valid) {
           a.part_ml[2 * prow] = m;
@@ -511,14 +536,6 @@ int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
   constexpr int smem = (int)smem_bytes<HDC>();
   static_assert(smem <= 227 * 1024, "shared memory");
   PE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  {
-    // the warpgroups' register re-split assumes the launch grants 168 per thread:
-    // with fewer, setmaxnreg.inc would wait for registers that never free up
-    cudaFuncAttributes fa;
-    PE_CUDA_TRY(cudaFuncGetAttributes(&fa, kern));
-    PE_CHECK_ARG(fa.numRegs * kThreads >= 128 * kRegsLow + 256 * kRegsHigh,
-                 "attn_paged: kernel compiled with too few registers");
-  }
   const int o_vec = (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 && a.o_ld % 8 == 0;
   return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, tk, tv, a, box,
                        o_vec);
