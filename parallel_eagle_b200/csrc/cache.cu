@@ -24,8 +24,9 @@ namespace {
 // its share of the three flat index spaces -- new rows, pages taken, pages given back --
 // finding an index's request by bisection in shared memory.  A row's page comes straight
 // from the ring when this call is the one that takes it, so no block reads what another
-// writes and one launch does it all.  Bound by launch latency up to some 100K rows, by the
-// 16 bytes written per row above.
+// writes and one launch does it all.  A thread describes two rows (one bisection, 16-byte
+// stores).  Bound by launch latency up to some 100K rows, by the 16 bytes written per row
+// above.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanBatch = 8192;  // requests whose scan fits the block's shared memory
 
@@ -49,7 +50,7 @@ __device__ __forceinline__ int find(const int* v, int n, int x) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
+plan_kernel(int B, int64_t width, int N, int page, int64_t rows, int sp,
             const int32_t* __restrict__ lens, const int32_t* __restrict__ want,
             int32_t* table, int64_t table_ld, int32_t* ring_pages,
             const int64_t* __restrict__ ring, int64_t* __restrict__ ring_out,
@@ -59,6 +60,8 @@ plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
   int* s_cu = sm;                  // [B + 1] first new row
   int* s_grow = s_cu + B + 1;      // [B + 1] pages taken by the requests before
   int* s_drop = s_grow + B + 1;    // [B + 1] pages given back by the requests before
+  int* s_used = s_drop + B + 1;    // [B] pages held; -1: the lengths fit no table
+  int* s_from = s_used + B;        // [B] keys held
   __shared__ Scan3 s_warp[kPlanThreads / 32];
   __shared__ int s_refused, s_taken, s_given;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -66,17 +69,11 @@ plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
   const int64_t head = ring[0], tail = ring[1];
   // counters that no ring of N pages can have serve nothing
   const bool sane = head >= 0 && tail >= head && tail - head <= N;
-  const int64_t avail = sane ? tail - head : 0, room = sane ? N - avail : 0;
-
-  // used / need of request b; false when the lengths are not served by the table at all
-  auto pages_of = [&](int b, int& from, int& to, int& used, int& need) {
-    from = lens[b];
-    to = want[b];
-    const bool fits = from >= 0 && to >= 0 && (to + (int64_t)page - 1) / page <= width &&
-                      (from + (int64_t)page - 1) / page <= width;
-    used = fits ? max((int)(((int64_t)from + page - 1) / page), sp) : 0;
-    need = fits ? max((int)(((int64_t)to + page - 1) / page), sp) : 0;
-    return fits;
+  const int avail = sane ? (int)(tail - head) : 0, room = sane ? N - avail : 0;
+  const uint32_t head_at = sane ? (uint32_t)(head % N) : 0, tail_at = sane ? (uint32_t)(tail % N) : 0;
+  auto ring_at = [&](uint32_t first, uint32_t i) {  // i < N
+    const uint32_t x = first + i;
+    return x >= (uint32_t)N ? x - (uint32_t)N : x;
   };
 
   // ---- exclusive scan of (new rows, pages taken, pages given back) over the requests ----
@@ -84,13 +81,17 @@ plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
   for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     Scan3 v{0, 0, 0};
-    int from = 0, to = 0, used = 0, need = 0;
     if (b < B) {
-      pages_of(b, from, to, used, need);
+      const int from = lens[b], to = want[b];
+      const int64_t u = ((int64_t)from + page - 1) / page, n = ((int64_t)to + page - 1) / page;
+      const bool fits = from >= 0 && to >= 0 && u <= width && n <= width;
+      const int used = max((int)u, sp), need = max((int)n, sp);
+      s_from[b] = from;
+      s_used[b] = fits ? used : -1;
       // (lengths the table cannot hold still own their rows, without slots)
       v.rows = max((int64_t)0, (int64_t)to - from);
-      v.grow = max(0, need - used);
-      v.drop = max(0, used - need);
+      v.grow = fits ? max(0, need - used) : 0;
+      v.drop = fits ? max(0, used - need) : 0;
     }
     Scan3 inc = v;
 #pragma unroll
@@ -122,18 +123,17 @@ plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
 
   // a request is served when its pages are there: growth while the ring's pages last,
   // returns while the ring has room (it always has, unless a page was given back twice)
-  auto served = [&](int b, bool fits) {
+  auto served = [&](int b) {
     const bool grows = s_grow[b + 1] > s_grow[b], drops = s_drop[b + 1] > s_drop[b];
-    return fits && (!grows || s_grow[b + 1] <= avail) && (!drops || s_drop[b + 1] <= room);
+    return s_used[b] >= 0 && (!grows || s_grow[b + 1] <= avail) && (!drops || s_drop[b + 1] <= room);
   };
 
   if (blockIdx.x == 0) {
     for (int b = tid; b < B; b += kPlanThreads) {
-      int from, to, used, need;
-      const bool ok = served(b, pages_of(b, from, to, used, need));
-      granted[b] = ok ? to : from;
-      if (ok && need > used) atomicAdd(&s_taken, need - used);
-      if (ok && used > need) atomicAdd(&s_given, used - need);
+      const bool ok = served(b);
+      granted[b] = ok ? want[b] : s_from[b];
+      if (ok && s_grow[b + 1] > s_grow[b]) atomicAdd(&s_taken, s_grow[b + 1] - s_grow[b]);
+      if (ok && s_drop[b + 1] > s_drop[b]) atomicAdd(&s_given, s_drop[b + 1] - s_drop[b]);
       if (!ok) atomicAdd(&s_refused, 1);
     }
     for (int b = tid; b <= B; b += kPlanThreads) cu[b] = s_cu[b];
@@ -146,37 +146,48 @@ plan_kernel(int B, int64_t width, int64_t N, int page, int64_t rows, int sp,
   }
 
   const int64_t stride = (int64_t)gridDim.x * kPlanThreads, i0 = (int64_t)blockIdx.x * kPlanThreads + tid;
-  // ---- new rows: position and slot ----
-  for (int64_t r = i0; r < rows; r += stride) {
-    int64_t slot = -1, p = 0;
-    if (r < s_cu[B]) {
-      const int b = find(s_cu, B, (int)r);
-      int from, to, used, need;
-      const bool ok = served(b, pages_of(b, from, to, used, need));
-      p = (int64_t)from + (int)r - s_cu[b];
-      if (ok) {
-        const int64_t i = p / page;
-        const int id = i >= used ? ring_pages[(head + s_grow[b] + i - used) % N]
-                                 : table[(int64_t)b * table_ld + i];
-        slot = (int64_t)id * page + p % page;
+  // ---- new rows, two a thread: position and slot ----
+  const int live = s_cu[B];
+  const bool wide = ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(pos)) & 15u) == 0;
+  for (int64_t r0 = 2 * i0; r0 < rows; r0 += 2 * stride) {
+    int64_t slot[2] = {-1, -1}, p[2] = {0, 0};
+    int b = r0 < live ? find(s_cu, B, (int)r0) : 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t r = r0 + e;
+      if (r >= live) break;
+      while (r >= s_cu[b + 1]) ++b;  // (requests without rows)
+      p[e] = (int64_t)s_from[b] + ((int)r - s_cu[b]);
+      if (!served(b)) continue;
+      const uint32_t i = (uint32_t)p[e] / (uint32_t)page;
+      const int id = i >= (uint32_t)s_used[b]
+                         ? ring_pages[ring_at(head_at, s_grow[b] + i - s_used[b])]
+                         : table[(int64_t)b * table_ld + i];
+      slot[e] = (int64_t)id * page + ((uint32_t)p[e] - i * (uint32_t)page);
+    }
+    if (wide && r0 + 1 < rows) {
+      *reinterpret_cast<longlong2*>(slots + r0) = make_longlong2(slot[0], slot[1]);
+      *reinterpret_cast<longlong2*>(pos + r0) = make_longlong2(p[0], p[1]);
+    } else {
+      for (int e = 0; e < 2 && r0 + e < rows; ++e) {
+        slots[r0 + e] = slot[e];
+        pos[r0 + e] = p[e];
       }
     }
-    slots[r] = slot;
-    pos[r] = p;
   }
   // ---- pages taken: table entries ----
-  for (int64_t g = i0; g < min((int64_t)s_grow[B], avail); g += stride) {
+  for (int64_t g = i0; g < min(s_grow[B], avail); g += stride) {
     const int b = find(s_grow, B, (int)g);
-    int from, to, used, need;
-    if (!served(b, pages_of(b, from, to, used, need))) continue;
-    table[(int64_t)b * table_ld + used + (int)g - s_grow[b]] = ring_pages[(head + g) % N];
+    if (served(b))
+      table[(int64_t)b * table_ld + s_used[b] + (int)g - s_grow[b]] =
+          ring_pages[ring_at(head_at, (uint32_t)g)];
   }
   // ---- pages given back: ring entries ----
-  for (int64_t d = i0; d < min((int64_t)s_drop[B], room); d += stride) {
+  for (int64_t d = i0; d < min(s_drop[B], room); d += stride) {
     const int b = find(s_drop, B, (int)d);
-    int from, to, used, need;
-    if (!served(b, pages_of(b, from, to, used, need))) continue;
-    ring_pages[(tail + d) % N] = table[(int64_t)b * table_ld + need + (int)d - s_drop[b]];
+    if (served(b))
+      ring_pages[ring_at(tail_at, (uint32_t)d)] =
+          table[(int64_t)b * table_ld + s_used[b] - (s_drop[b + 1] - s_drop[b]) + (int)d - s_drop[b]];
   }
 }
 
@@ -258,7 +269,7 @@ extern "C" int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_
   PE_CHECK_ARG(width >= 1 && width * page < (1ll << 31) && table_ld >= width,
                "cache_plan: block table of %lld pages (row stride %lld)", (long long)width,
                (long long)table_ld);
-  PE_CHECK_ARG(num_pages >= 1 && num_pages < (1ll << 31) && B * width < (1ll << 31),
+  PE_CHECK_ARG(num_pages >= 1 && num_pages < (1ll << 30) && B * width < (1ll << 31),
                "cache_plan: %lld pages", (long long)num_pages);
   PE_CHECK_ARG(rows >= 0 && rows < (1ll << 31), "cache_plan: %lld new rows", (long long)rows);
   PE_CHECK_ARG(shared >= 0 && shared % page == 0 && shared / page <= width,
@@ -268,15 +279,18 @@ extern "C" int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_
                "cache_plan: null pointer");
   PE_CHECK_ARG(ring != ring_out && lens != granted && new_lens != granted,
                "cache_plan: ring_out and granted must not alias the inputs");
-  const size_t smem = 3 * (size_t)(B + 1) * sizeof(int);
+  const size_t smem = (5 * (size_t)B + 3) * sizeof(int);
   if (smem > 48 * 1024)
     PE_CUDA_TRY(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)smem));
-  // a block per 1024 rows (and per 256 requests, whose pages it fills), up to one per SM
+  // a block per 1024 rows (and per 256 requests, whose pages it fills), up to three per SM:
+  // a row's chain of dependent reads takes the time, so the more in flight the better
+  // (512 prompts, 811K rows: 14 us with three, 23 us with one and a row a thread)
   const int64_t want = std::max(ceil_div(rows, 2 * kPlanThreads), ceil_div(B, 256));
-  const int blocks = (int)std::min<int64_t>(std::max<int64_t>(want, 1), sm_count());
+  const int64_t most = smem > 64 * 1024 ? 1 : 3;
+  const int blocks = (int)std::min<int64_t>(std::max<int64_t>(want, 1), most * sm_count());
   plan_kernel<<<blocks, kPlanThreads, smem, as_stream(stream)>>>(
-      (int)B, width, num_pages, (int)page, rows, (int)(shared / page), lens, new_lens, table,
+      (int)B, width, (int)num_pages, (int)page, rows, (int)(shared / page), lens, new_lens, table,
       table_ld, free_ring, ring, ring_out, granted, cu, slots, pos);
   PE_LAUNCHED();
   return PE_OK;
