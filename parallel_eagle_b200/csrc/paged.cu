@@ -15,24 +15,46 @@ namespace {
 
 // ------------------------------------------------------------- CUDA-core kernel ----
 // A block holds 16 packed rows (fp32) and walks its key tiles, 32 keys at a time, through
-// shared memory; 8 threads share a row's scores, statistics and output columns.  It serves
-// fp32 (whose products the tensor cores would round) and what the tensor-core kernels do
-// not take.  Bound by shared-memory reads: a key's element is read once per 4 rows of a
-// warp for the scores and once for the output.
+// two shared-memory buffers: the next tile's copies run while this one is computed.  8
+// threads share a row's scores, statistics and output columns.  It serves fp32 (whose
+// products the tensor cores would round) and what the tensor-core kernels do not take.
+// Bound by shared-memory reads: a key's element is read once per 4 rows of a warp for the
+// scores and once for the output.
 constexpr int kThreads = 128;
 constexpr int kSimtRows = 16;
 constexpr int kTK = 32;
+constexpr int kLdP = kTK + 8;  // a warp's four rows of probabilities in different banks
+
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  return make_float4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+
+// shared-memory row of a K or V tile, in elements: padded so that 8 keys' 16-byte (fp32)
+// or 8-byte (bf16) pieces fall into different banks
+__host__ __device__ constexpr int simt_ld(int hdp, int es) { return hdp + 16 / es; }
+inline size_t simt_smem(int hdp, int es) {
+  return 4ull * kTK * simt_ld(hdp, es) * es + (size_t)kSimtRows * (hdp + 4 + kLdP) * sizeof(float);
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
   constexpr int Mt = kSimtRows;
-  extern __shared__ float sm[];
-  const int ldk = hdp + 4;
-  float* sQ = sm;                 // [Mt][ldk]
-  float* sK = sQ + Mt * ldk;      // [kTK][ldk]
-  float* sV = sK + kTK * ldk;     // [kTK][ldk]
-  float* sP = sV + kTK * ldk;     // [Mt][kTK]
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int ldk = simt_ld(hdp, sizeof(T)), ldq = hdp + 4;
+  T* sKV = reinterpret_cast<T*>(smem);  // [buffer][K, V][kTK][ldk]
+  float* sQ = reinterpret_cast<float*>(sKV + 4 * kTK * ldk);  // [Mt][ldq]
+  float* sP = sQ + Mt * ldq;                                  // [Mt][kLdP]
   __shared__ int64_t scratch[kThreads / 32 + 4];
   const int tid = threadIdx.x, r = tid >> 3, c = tid & 7;
   const T* q = static_cast<const T*>(a.q);
@@ -50,16 +72,53 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
     const int rr = w.rt * Mt + r;  // this thread's packed row
     const bool valid = r < rows;
     const int64_t lim = valid ? w.limit(rr) : 0;
-    __syncthreads();  // the tile before is read
-    for (int i = tid; i < Mt * hdp; i += kThreads) {
-      const int ri = i / hdp, d = i - ri * hdp;
-      float x = 0.f;
-      if (ri < rows && d < a.hd) {
-        const int pr = w.rt * Mt + ri;
-        x = to_f(q[(int64_t)(w.rq.row0 + pr / a.G) * a.q_ld +
-                   (int64_t)(w.kvh * a.G + pr % a.G) * a.hd + d]);
+    // start the copies of tile t (zeros behind the last key and outside the pool)
+    auto fetch = [&](int t) {
+      const int key = tid >> 2, part = tid & 3;
+      const int64_t at = a.kbeg + (int64_t)t * kTK + key;
+      const T *kr = kc, *vr = vc;
+      bool live = false;
+      if (at < w.kend) {
+        const int64_t pi = div_pos(at, a.page);
+        const int id = w.pages()[pi];
+        if (id >= 0 && id < a.num_pages) {
+          const int64_t off = (((int64_t)id * a.Hkv + w.kvh) * a.page + (at - pi * a.page)) * a.hd;
+          kr = kc + off;
+          vr = vc + off;
+          live = true;
+        }
       }
-      sQ[ri * ldk + d] = x;
+      T* dk = sKV + (t & 1) * 2 * kTK * ldk + key * ldk;
+      T* dv = dk + kTK * ldk;
+      if (vec) {
+        constexpr int N = 16 / sizeof(T);
+        for (int u = part * N; u < hdp; u += 4 * N) {
+          copy16(dk + u, kr + u, live);
+          copy16(dv + u, vr + u, live);
+        }
+      } else {
+        for (int d = part; d < hdp; d += 4) {
+          dk[d] = live && d < a.hd ? kr[d] : from_f<T>(0.f);
+          dv[d] = live && d < a.hd ? vr[d] : from_f<T>(0.f);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();  // the segment before is read
+    if (w.t0 < w.t1) fetch(w.t0);
+    {
+      const int tok = rr / a.G;
+      const T* qr = q + (int64_t)(w.rq.row0 + tok) * a.q_ld +
+                    (int64_t)(w.kvh * a.G + rr - tok * a.G) * a.hd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = 4 * (c + 8 * i);
+        if (d >= hdp) break;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = valid && d + e < a.hd ? to_f(qr[d + e]) : 0.f;
+        *reinterpret_cast<float4*>(sQ + r * ldq + d) = make_float4(x[0], x[1], x[2], x[3]);
+      }
     }
     float4 acc[8];
 #pragma unroll
@@ -67,53 +126,18 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
     float m = -INFINITY, l = 0.f;
     for (int t = w.t0; t < w.t1; ++t) {
       const int64_t k0 = a.kbeg + (int64_t)t * kTK;
-      // keys of the tile -> shared memory (zeros behind the last one)
-      {
-        const int key = tid >> 2, part = tid & 3;
-        const int64_t at = k0 + key;
-        const T *kr = nullptr, *vr = nullptr;
-        if (at < w.kend) {
-          const int64_t pi = at / a.page;
-          const int id = w.pages()[pi];
-          if (id >= 0 && id < a.num_pages) {
-            const int64_t off = (((int64_t)id * a.Hkv + w.kvh) * a.page + (at - pi * a.page)) * a.hd;
-            kr = kc + off;
-            vr = vc + off;
-          }
-        }
-        float* dk = sK + key * ldk;
-        float* dv = sV + key * ldk;
-        if (vec) {
-          constexpr int N = 16 / sizeof(T);
-          for (int u = part; u < hdp / N; u += 4) {
-            uint4 ku = make_uint4(0, 0, 0, 0), vu = ku;
-            if (kr) {
-              ku = reinterpret_cast<const uint4*>(kr)[u];
-              vu = reinterpret_cast<const uint4*>(vr)[u];
-            }
-            const T* kt = reinterpret_cast<const T*>(&ku);
-            const T* vt = reinterpret_cast<const T*>(&vu);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-              dk[u * N + e] = to_f(kt[e]);
-              dv[u * N + e] = to_f(vt[e]);
-            }
-          }
-        } else {
-          for (int d = part; d < hdp; d += 4) {
-            const bool in = kr && d < a.hd;
-            dk[d] = in ? to_f(kr[d]) : 0.f;
-            dv[d] = in ? to_f(vr[d]) : 0.f;
-          }
-        }
-      }
-      __syncthreads();
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncthreads();  // tile t is here, tile t - 1 is read
+      if (t + 1 < w.t1) fetch(t + 1);
+      const T* sK = sKV + (t & 1) * 2 * kTK * ldk;
+      const T* sV = sK + kTK * ldk;
       float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
       for (int d = 0; d < hdp; d += 4) {
-        const float4 qv = *reinterpret_cast<const float4*>(sQ + r * ldk + d);
+        const float4 qv = load4(sQ + r * ldq + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 kv = *reinterpret_cast<const float4*>(sK + (c + 8 * i) * ldk + d);
+          const float4 kv = load4(sK + (c + 8 * i) * ldk + d);
           s[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[i]))));
         }
       }
@@ -133,7 +157,7 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
       for (int i = 0; i < 4; ++i) {
         const float p = exp2f(s[i] - m_use);
         rs += p;
-        sP[r * kTK + c + 8 * i] = p;
+        sP[r * kLdP + c + 8 * i] = p;
       }
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) rs += __shfl_xor_sync(0xffffffffu, rs, o);
@@ -145,19 +169,20 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
         if (c + 8 * i >= groups) break;
         float4 o = acc[i];
         o.x *= alpha; o.y *= alpha; o.z *= alpha; o.w *= alpha;
-        const float* vcol = sV + 4 * (c + 8 * i);
-#pragma unroll 8
-        for (int kk = 0; kk < kTK; ++kk) {
-          const float p = sP[r * kTK + kk];
-          const float4 v = *reinterpret_cast<const float4*>(vcol + kk * ldk);
-          o.x = fmaf(p, v.x, o.x);
-          o.y = fmaf(p, v.y, o.y);
-          o.z = fmaf(p, v.z, o.z);
-          o.w = fmaf(p, v.w, o.w);
+        const T* vcol = sV + 4 * (c + 8 * i);
+#pragma unroll 2
+        for (int kk = 0; kk < kTK; kk += 4) {
+          const float4 p = load4(sP + r * kLdP + kk);
+          const float4 v0 = load4(vcol + kk * ldk), v1 = load4(vcol + (kk + 1) * ldk);
+          const float4 v2 = load4(vcol + (kk + 2) * ldk), v3 = load4(vcol + (kk + 3) * ldk);
+          o.x = fmaf(p.w, v3.x, fmaf(p.z, v2.x, fmaf(p.y, v1.x, fmaf(p.x, v0.x, o.x))));
+          o.y = fmaf(p.w, v3.y, fmaf(p.z, v2.y, fmaf(p.y, v1.y, fmaf(p.x, v0.y, o.y))));
+          o.z = fmaf(p.w, v3.z, fmaf(p.z, v2.z, fmaf(p.y, v1.z, fmaf(p.x, v0.z, o.z))));
+          o.w = fmaf(p.w, v3.w, fmaf(p.z, v2.w, fmaf(p.y, v1.w, fmaf(p.x, v0.w, o.w))));
         }
         acc[i] = o;
       }
-      __syncthreads();
+      __syncwarp();
     }
     if (a.pre_lse && !joined) {
       wait_kernel_before();  // the prefix's rows
@@ -211,119 +236,92 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
 }
 
 // ---------------------------------------------------------------------- join ----
-// Block (c, y): joins the pieces of the entity that starts in block c, rows 4y .. 4y + 3.
-// Pieces are weighted with 2^(m_i - max m) and added in a fixed order.  A warp joins a row;
-// when an entity lies in many pieces (a few long requests over all SMs) the four warps
-// share each row's pieces instead, as one warp's loads would run one after another.
-constexpr int kJoinThreads = 128;
+// Block (c, y): joins the pieces of the entity that starts in block c, rows 4y .. 4y + 3, a
+// warp a row.  Pieces are weighted with 2^(m_i - max m) and added in piece order, eight
+// loads in flight.  Bound by latency: most blocks have nothing to join, the others read
+// three things one after another (what to join, its statistics, its accumulators).  (Blocks
+// of 1024 threads, or four warps a row, took 1.3 to 1.5 times as long.)
 constexpr int kJoinRows = 4;
-constexpr int kJoinSplit = 16;  // pieces from which the warps share a row
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(32 * kJoinRows)
 paged_join_kernel(const __grid_constant__ Args a, int Mt) {
-  extern __shared__ float sw[];  // [warps][blocks] weights
-  __shared__ float sums[kJoinRows][256];
   start_next_kernel();
   wait_kernel_before();
   const Open op = a.open[blockIdx.x];
-  const int row_base = blockIdx.y * kJoinRows;
-  if (op.parts == 0 || row_base >= op.rows) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, row = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
+  if (op.parts == 0 || row >= op.rows) return;
   constexpr int E = 256 / 32;  // elements per lane, in runs of V
-  const bool share = op.parts > kJoinSplit;
-  float* wgt = sw + warp * gridDim.x;
-
-  for (int k = 0; k < (share ? kJoinRows : 1); ++k) {
-    const int row = row_base + (share ? k : warp);
-    if (row >= op.rows) break;
-    auto slot_row = [&](int i) {
-      const int s = i == 0 ? op.slot : 2 * ((int)blockIdx.x + i);
-      return (int64_t)s * Mt + row;
-    };
-    auto column = [&](int e) { return (e / V) * (32 * V) + lane * V + e % V; };
-    float mx = -INFINITY;
-    for (int i = lane; i < op.parts; i += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot_row(i));
-      if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
-    }
-    mx = warp_max(mx);
-    float l = 0.f;
-    for (int i = lane; i < op.parts; i += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot_row(i));
-      const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
-      wgt[i] = w;
-      l += ml.y == 0.f ? 0.f : w * ml.y;
-    }
-    l = warp_sum(l);
-    __syncwarp();
-    float acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = share ? warp : 0; i < op.parts; i += share ? kJoinRows : 1) {
-      const float w = wgt[i];
-      const float* src = a.part_o + slot_row(i) * a.hd;
-#pragma unroll
-      for (int e = 0; e < E; e += V) {
-        if (column(e) >= a.hd) continue;
-        float v[V];
-        if constexpr (V == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src + column(e));
-          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-          v[0] = src[column(e)];
-        }
-        // (a piece without keys left its accumulator unwritten)
-#pragma unroll
-        for (int q = 0; q < V; ++q) acc[e + q] += w == 0.f ? 0.f : w * v[q];
-      }
-    }
-    if (share) {
-      if (k > 0) __syncthreads();  // the row before is read
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (column(e) < a.hd) sums[warp][column(e)] = acc[e];
-      __syncthreads();
-      if (warp != 0) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (column(e) < a.hd)
-          acc[e] = (sums[0][column(e)] + sums[1][column(e)]) +
-                   (sums[2][column(e)] + sums[3][column(e)]);
-    }
-    const int rr = op.r0 + row;
-    const int tok = op.row0 + rr / a.G, head = op.kvh * a.G + rr % a.G;
-    const RowScale f = finish_row(a, tok, head, mx, l);
-    const int64_t at = ((int64_t)tok * a.Hq + head) * a.hd;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = column(e);
-      if (d >= a.hd) continue;
-      float x = f.own == 0.f ? 0.f : acc[e] * f.own;
-      if (f.pre != 0.f) x += f.pre * a.pre_o[at + d];
-      if (a.o32)
-        a.o32[at + d] = x;
-      else
-        static_cast<T*>(a.o)[(int64_t)tok * a.o_ld + (int64_t)head * a.hd + d] = from_f<T>(x);
-    }
-    if (lane == 0) a.lse[(int64_t)head * a.T + tok] = f.lse;
+  auto slot_row = [&](int i) {
+    const int s = i == 0 ? op.slot : 2 * ((int)blockIdx.x + i);
+    return (int64_t)s * Mt + row;
+  };
+  auto stat = [&](int i) { return *reinterpret_cast<const float2*>(a.part_ml + 2 * slot_row(i)); };
+  auto column = [&](int e) { return (e / V) * (32 * V) + lane * V + e % V; };
+  float mx = -INFINITY, l = 0.f;
+  for (int i = lane; i < op.parts; i += 32) {
+    const float2 ml = stat(i);
+    if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
   }
+  mx = warp_max(mx);
+  for (int i = lane; i < op.parts; i += 32) {
+    const float2 ml = stat(i);
+    l += ml.y == 0.f ? 0.f : exp2f(ml.x - mx) * ml.y;
+  }
+  l = warp_sum(l);
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < op.parts; ++i) {
+    const float2 ml = stat(i);
+    const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - mx);
+    const float* src = a.part_o + slot_row(i) * a.hd;
+#pragma unroll
+    for (int e = 0; e < E; e += V) {
+      if (column(e) >= a.hd) continue;
+      float v[V];
+      if constexpr (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src + column(e));
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+      } else {
+        v[0] = src[column(e)];
+      }
+      // (a piece without keys left its accumulator unwritten)
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[e + q] += w == 0.f ? 0.f : w * v[q];
+    }
+  }
+  const int rr = op.r0 + row;
+  const int tok = op.row0 + rr / a.G, head = op.kvh * a.G + rr % a.G;
+  const RowScale f = finish_row(a, tok, head, mx, l);
+  const int64_t at = ((int64_t)tok * a.Hq + head) * a.hd;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = column(e);
+    if (d >= a.hd) continue;
+    float x = f.own == 0.f ? 0.f : acc[e] * f.own;
+    if (f.pre != 0.f) x += f.pre * a.pre_o[at + d];
+    if (a.o32)
+      a.o32[at + d] = x;
+    else
+      static_cast<T*>(a.o)[(int64_t)tok * a.o_ld + (int64_t)head * a.hd + d] = from_f<T>(x);
+  }
+  if (lane == 0) a.lse[(int64_t)head * a.T + tok] = f.lse;
 }
 
 int launch_join(int dtype, const Args& a, int blocks, int Mt, cudaStream_t st) {
-  const size_t smem = (size_t)blocks * (kJoinThreads / 32) * sizeof(float);
   const dim3 grid((unsigned)blocks, (unsigned)ceil_div(Mt, kJoinRows));
   return PE_DISPATCH(dtype, T, [&]() -> int {
     auto kern = a.hd % 4 == 0 ? paged_join_kernel<T, 4> : paged_join_kernel<T, 1>;
-    return launch_kernel(kern, grid, kJoinThreads, smem, st, true, a, Mt);
+    return launch_kernel(kern, grid, 32 * kJoinRows, 0, st, true, a, Mt);
   });
 }
 
 int launch_simt(int dtype, const Args& a, int blocks, bool dependent, cudaStream_t st) {
-  const int hdp = (a.hd + 3) / 4 * 4;
-  const size_t smem = (size_t)((kSimtRows + 2 * kTK) * (hdp + 4) + kSimtRows * kTK) * sizeof(float);
   const int es = dtype == PE_F32 ? 4 : 2;
+  const int hdp = (a.hd + 3) / 4 * 4;
+  const size_t smem = simt_smem(hdp, es);
   const int vec = a.hd * es % 16 == 0 && (reinterpret_cast<uintptr_t>(a.kc) & 15u) == 0 &&
                   (reinterpret_cast<uintptr_t>(a.vc) & 15u) == 0;
   return PE_DISPATCH(dtype, T, [&]() -> int {
@@ -341,7 +339,11 @@ struct Phase {
   int Mt, blocks;
 };
 
-Phase simt_phase(int hd) { return {kSimt, kSimtRows, sm_count() * (hd <= 128 ? 4 : 2)}; }
+Phase simt_phase(int dtype, int hd) {
+  // as many blocks as the tiles' shared memory lets an SM hold, four at most
+  const size_t smem = simt_smem((hd + 3) / 4 * 4, dtype == PE_F32 ? 4 : 2);
+  return {kSimt, kSimtRows, sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, 220 * 1024 / smem))};
+}
 
 // tensor-core kernel for `rows` packed rows (on average) per request and KV head
 Phase tc_phase(int64_t rows) {
@@ -393,10 +395,10 @@ extern "C" size_t pe_attn_paged_workspace(int dtype, int64_t B, int64_t T, int H
                                           int64_t shared) {
   if (B < 1 || T < 1 || Hq < 1 || Hkv < 1 || hd < 1) return 0;
   const int64_t G = std::max(Hq / Hkv, 1);
-  int64_t bytes = phase_bytes(simt_phase(hd), hd);  // (operands may rule the tensor cores out)
+  int64_t bytes = phase_bytes(simt_phase(dtype, hd), hd);  // (operands may rule the tensor cores out)
   if (tc_sizes(dtype, hd)) bytes = std::max(bytes, phase_bytes(tc_phase(ceil_div(T * G, B)), hd));
   if (shared <= 0) return (size_t)bytes;
-  int64_t prefix = phase_bytes(simt_phase(hd), hd);
+  int64_t prefix = phase_bytes(simt_phase(dtype, hd), hd);
   if (tc_sizes(dtype, hd)) prefix = std::max(prefix, phase_bytes(tc_phase(T * G), hd));
   return (size_t)(al256(T * Hq * hd * 4) + al256(T * Hq * 4) + prefix + bytes);
 }
@@ -459,7 +461,7 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     ws += al256(T * Hq * hd * 4);
     float* pre_lse = reinterpret_cast<float*>(ws);
     ws += al256(T * Hq * 4);
-    const Phase p = tc ? tc_phase(T * a.G) : simt_phase(hd);
+    const Phase p = tc ? tc_phase(T * a.G) : simt_phase(dtype, hd);
     Args pa = a;
     pa.all_rows = 1;
     pa.kmax = shared;
@@ -473,7 +475,7 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     a.pre_o = pre_o;
     a.pre_lse = pre_lse;
   }
-  const Phase p = tc ? tc_phase(ceil_div(T * a.G, B)) : simt_phase(hd);
+  const Phase p = tc ? tc_phase(ceil_div(T * a.G, B)) : simt_phase(dtype, hd);
   carve(a, p, ws);
   return run_phase(dtype, p, a, shared > 0, st);
 }
