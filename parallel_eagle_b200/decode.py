@@ -32,7 +32,10 @@ def propose_tree(drafter, context_ids: torch.Tensor, context_feats: torch.Tensor
     if k <= 0:
         return [], []
     vals, toks = ops.topk_logprobs(logits[pending:], beam_width)
-    vals, toks = vals.tolist(), toks.tolist()
+    return _grow_tree(vals.tolist(), toks.tolist(), k, beam_width)
+
+
+def _grow_tree(vals, toks, k: int, beam_width: int) -> tuple[list[int], list[int]]:
     beam: list[tuple[int, float]] = [(-1, 0.0)]  # (parent node index, cumulative logprob)
     node_tokens: list[int] = []
     parents: list[int] = []
@@ -55,6 +58,33 @@ def propose_chain(drafter, context_ids: torch.Tensor, context_feats: torch.Tenso
         return []
     _, toks = ops.topk_logprobs(logits[pending:], 1, raw=True)
     return [int(t) for t in toks[:, 0].tolist()]
+
+
+def propose_trees(drafter, cache, ids: torch.Tensor, feats: torch.Tensor, news: list[int],
+                  k: int, top_k: int, max_nodes: int) -> list[tuple[list[int], list[int]]]:
+    """:func:`propose_tree` for every request of a :class:`cache.DraftCache` that has new
+    confirmed tokens (``news[b]`` of them, in ``ids`` and ``feats`` one request after
+    another): one drafter pass over the new tokens and prediction slots of all requests,
+    one selection launch."""
+    if k <= 0:
+        raise ValueError(f"k must be positive, got {k}")
+    logits = drafter.draft_logits_cached(cache, ids, feats, news, k)
+    beam_width = max(1, min(top_k, max_nodes // k))
+    vals, toks = ops.topk_logprobs(logits.flatten(0, 1), beam_width)
+    shape = (logits.shape[0], k, beam_width)
+    return [_grow_tree(v, t, k, beam_width)
+            for v, t in zip(vals.view(shape).tolist(), toks.view(shape).tolist())]
+
+
+def propose_chains(drafter, cache, ids: torch.Tensor, feats: torch.Tensor, news: list[int],
+                   k: int) -> list[list[int]]:
+    """:func:`propose_chain` for every request of a :class:`cache.DraftCache` that has new
+    confirmed tokens: one drafter pass and one selection launch for all of them."""
+    if k <= 0:
+        raise ValueError(f"k must be positive, got {k}")
+    logits = drafter.draft_logits_cached(cache, ids, feats, news, k)
+    _, toks = ops.topk_logprobs(logits.flatten(0, 1), 1, raw=True)
+    return toks.view(-1, k).tolist()
 
 
 def propose_chain_sequential(drafter, context_ids: torch.Tensor, context_feats: torch.Tensor,

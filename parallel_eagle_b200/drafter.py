@@ -177,6 +177,75 @@ class ParallelDrafter(nn.Module):
         return linear(hidden[p - 1 :], self._lm_head[0].weight)
 
     @torch.no_grad()
+    def forward_cached(self, cache, ids: torch.Tensor, feats: torch.Tensor, news: list[int],
+                       k: int) -> tuple[torch.Tensor, list[int]]:
+        """Append ``news[b]`` confirmed tokens to request b of a :class:`cache.DraftCache` and
+        run them, each request's followed by its ``k - 1`` prediction slots.  ``ids`` and
+        ``feats`` hold the tokens of all requests one after another; a request without new
+        tokens is left out.  Returns the final hidden states ``(rows, H)`` and each
+        request's first row in them (one entry more than requests).
+
+        The rows see their request's cached keys and the rows before them: the partition
+        layout with ``(a0, a1, K) = (p - 1, p, k)`` again, as the prediction slots follow the
+        last real one.  The prediction slots' keys are dropped afterwards."""
+        dev = self.device
+        if len(news) != cache.requests or min(news) < 0 or sum(news) != ids.shape[0] \
+                or feats.shape[0] != ids.shape[0]:
+            raise ValueError(f"{len(news)} counts of new tokens (sum {sum(news)}) for "
+                             f"{cache.requests} requests, {ids.shape[0]} tokens and "
+                             f"{feats.shape[0]} feature rows")
+        if k < 1 or ids.shape[0] == 0:
+            raise ValueError("drafting needs new tokens and k >= 1")
+        before = cache.lengths
+        first = [0]
+        real: list[int] = []  # rows of the confirmed tokens
+        for n in news:
+            real += range(first[-1], first[-1] + n)
+            first.append(first[-1] + (n + k - 1 if n else 0))
+        x = torch.empty(first[-1], self.hidden, dtype=self.param_dtype, device=dev)
+        if k > 1:
+            x[:] = self.mask_input(1)
+            x[torch.tensor(real).to(dev)] = self.real_input(ids.to(dev), feats.to(dev))
+        else:
+            x[:] = self.real_input(ids.to(dev), feats.to(dev))
+        cu, slots, pos = cache.resize([h + (n + k - 1 if n else 0) for h, n in zip(before, news)])
+        nh, nkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
+        for i, layer in enumerate(self.layers):
+            at = layer.attn
+            h, _ = ops.rmsnorm_fwd(x, layer.input_norm.weight, layer.input_norm.eps)
+            q, key, v = (ops.linear(h, m.weight) for m in (at.q_proj, at.k_proj, at.v_proj))
+            ops.rope_(q, nh, hd, pos, self.rope_theta)
+            ops.rope_(key, nkv, hd, pos, self.rope_theta)
+            with torch.cuda.device(dev):
+                ops.cache_append(key, v, slots, cache.k[i], cache.v[i])
+                if cache.shared:
+                    o, _ = ops.attn_paged_shared(q, cache.k[i], cache.v[i], cache.table,
+                                                 cache.lens, cu, cache.shared)
+                else:
+                    o, _ = ops.attn_paged(q, cache.k[i], cache.v[i], cache.table, cache.lens, cu)
+            x = ops.linear(o, at.o_proj.weight, residual=x)
+            h, _ = ops.rmsnorm_fwd(x, layer.post_norm.weight, layer.post_norm.eps)
+            w = torch.cat([layer.mlp.gate_proj.weight, layer.mlp.up_proj.weight], dim=0)
+            act = ops.swiglu_fwd(ops.linear(h, w), self.intermediate)
+            x = ops.linear(act, layer.mlp.down_proj.weight, residual=x)
+        if k > 1:
+            cache.resize([h + n for h, n in zip(before, news)])
+        fnorm = self._final_norm[0]
+        return ops.rmsnorm_fwd(x, fnorm.weight, fnorm.eps)[0], first
+
+    @torch.no_grad()
+    def draft_logits_cached(self, cache, ids: torch.Tensor, feats: torch.Tensor,
+                            news: list[int], k: int) -> torch.Tensor:
+        """:meth:`draft_logits` for a batch of requests whose context, all but the ``news[b]``
+        last confirmed tokens, is in ``cache``: logits ``(requests with new tokens, k, V)``
+        for the ``k`` tokens that follow each.  ``cache`` then holds those tokens too."""
+        hidden, first = self.forward_cached(cache, ids, feats, news, k)
+        rows = [first[b] + n - 1 + d for b, n in enumerate(news) if n for d in range(k)]
+        pick = torch.tensor(rows).to(hidden.device)
+        logits = linear(ops.gather_rows(hidden, pick), self._lm_head[0].weight)
+        return logits.view(-1, k, logits.shape[-1])
+
+    @torch.no_grad()
     def draft_logits_sequential(self, context_ids: torch.Tensor, context_feats: torch.Tensor,
                                 k: int) -> torch.Tensor:
         """Greedy drafting by ``k`` causal forward passes, each appending the previous

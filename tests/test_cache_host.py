@@ -93,3 +93,15 @@ def test_wrappers_refuse_host_tensors():
     for call in calls:
         with pytest.raises(_lib.PeError, match="CUDA tensors only"):
             call()
+
+
+def test_draft_cache_needs_a_gpu():
+    import types
+
+    from parallel_eagle_b200.cache import DraftCache
+
+    d = types.SimpleNamespace(device=torch.device("cpu"), param_dtype=torch.float32)
+    with pytest.raises(_lib.PeError, match="CUDA only"):
+        DraftCache(d, 1, 4)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        DraftCache(d, 1, 4, page=24)
