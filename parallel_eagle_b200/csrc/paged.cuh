@@ -88,7 +88,9 @@ struct Seg {
   int end;         // 1: no more segments
 };
 
-template <int Mt, int TK>
+// Mt: packed rows per tile.  TK: keys per tile.  kOver: what a segment's start and end cost
+// on top of its keys, in keys (Q rows in, result rows out, the pipeline's filling).
+template <int Mt, int TK, int kOver>
 struct Sched {
   const Args& a;
   int64_t total, per, pos, end;  // cost units; this block's piece is [pos, end)
@@ -122,15 +124,18 @@ struct Sched {
     r.R = (int)(((int64_t)r.n * a.G + Mt - 1) / Mt);
     return r;
   }
-  // cost of row tile rt: its keys times G, plus a key tile's worth for its start and end
+  // cost of row tile rt: its keys times G, plus the overhead.  (A last tile that is not full
+  // counts like any other: it waits as long for every key tile.)
   __device__ __forceinline__ int64_t cost(const Req& r, int rt) const {
-    return (r.A + TK) * a.G + (a.all_rows ? 0 : (int64_t)(rt + 1) * Mt);
+    return (r.A + kOver) * a.G + (a.all_rows ? 0 : (int64_t)(rt + 1) * Mt);
   }
+  // ... of the tiles before rt
   __device__ __forceinline__ int64_t cost_before(const Req& r, int64_t rt) const {
-    return rt * (r.A + TK) * a.G + (a.all_rows ? 0 : rt * (rt + 1) / 2 * Mt);
+    return rt * (r.A + kOver) * a.G + (a.all_rows ? 0 : rt * (rt + 1) / 2 * Mt);
   }
+  __device__ __forceinline__ int64_t head_cost(const Req& r) const { return cost_before(r, r.R); }
   __device__ __forceinline__ int64_t req_cost(const Req& r) const {
-    return (int64_t)a.Hkv * cost_before(r, r.R);
+    return (int64_t)a.Hkv * head_cost(r);
   }
 
   // all threads of the block; scratch: one int64 per warp plus 4
@@ -190,10 +195,10 @@ struct Sched {
       rq = request(++b);
       rc = req_cost(rq);
     }
-    const int64_t head_cost = cost_before(rq, rq.R);
+    const int64_t per_head = head_cost(rq);
     int64_t off = pos - base;
-    kvh = (int)div_pos(off, head_cost);
-    off -= kvh * head_cost;
+    kvh = (int)div_pos(off, per_head);
+    off -= kvh * per_head;
     // last row tile that starts at or before off
     int lo = 0, hi = rq.R;
     while (hi - lo > 1) {

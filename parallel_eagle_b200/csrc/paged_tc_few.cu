@@ -38,6 +38,7 @@ using namespace sm100;
 
 constexpr int kTile = 128;                    // keys per tile
 constexpr uint32_t kChunk = kTile * 128;      // 128 keys x 64 columns, 128-byte swizzled
+constexpr int kOver = 2 * kTile;              // a segment's start and end, in keys
 constexpr float kRaise = 8.f;                 // log2 of what a score may pass the bound by
 
 template <int N, int HDC>
@@ -185,7 +186,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     tmem_alloc(&sm.tmem, F::kTmem);
     tmem_relinquish();
   }
-  Sched<N, kTile> w(a);
+  Sched<N, kTile, kOver> w(a);
   w.init(sm.scratch);
   tc_fence_before();
   __syncthreads();

@@ -36,6 +36,7 @@ constexpr int kTile = 64;                     // keys per tile
 constexpr int kStages = 4;                    // K tiles, V tiles in shared memory
 constexpr uint32_t kChunk = kTile * 128;      // 64 keys x 64 columns, 128-byte swizzled
 constexpr uint32_t kQChunk = kHalf * 128;     // 128 rows x 64 columns
+constexpr int kOver = 4 * kTile;              // a segment's start and end, in keys
 constexpr float kRaise = 8.f;
 constexpr int kEmuEvery = 4;
 
@@ -56,6 +57,12 @@ constexpr size_t smem_bytes() {
 
 __device__ __forceinline__ uint32_t swz128(int r, int u) {
   return (uint32_t)(r * 128 + ((u ^ (r & 7)) << 4));
+}
+// 32 bytes, a whole sector, by one thread (rows lie one to a thread)
+__device__ __forceinline__ void st_v8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
@@ -113,7 +120,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tmem_alloc(&sm.tmem, 512);
     tmem_relinquish();
   }
-  Sched<kRows, kTile> w(a);
+  Sched<kRows, kTile, kOver> w(a);
   w.init(sm.scratch);
   tc_fence_before();
   __syncthreads();
@@ -297,16 +304,27 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         ok = mbar_wait(&sm.q_empty, (seq & 1) ^ 1u, status, 433);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        constexpr int U = HD / 8;
+        // unit u of rows r0, r0 + step, ...: the address moves on by heads, and to the next
+        // token's row where a group ends
+        constexpr int U = HD / 8, step = 64 / U;
         const int n = g.rows > kHalf ? kRows : kHalf;
-        for (int x = threadIdx.x - 64; x < n * U; x += 64) {
-          const int r = x / U, u = x % U;
+        const int u = (threadIdx.x - 64) % U;
+        int r = (threadIdx.x - 64) / U;
+        const int tok = (g.r0 + r) / a.G;
+        int rem = g.r0 + r - tok * a.G;
+        const __nv_bfloat16* src = q + (int64_t)(g.row0 + tok) * a.q_ld +
+                                   (int64_t)(g.kvh * a.G + rem) * HD + u * 8;
+        uint8_t* dst = sQ + (u >> 3) * kQChunk;
+#pragma unroll 8
+        for (; r < n; r += step) {
           const bool valid = r < g.rows;
-          const int pr = g.r0 + (valid ? r : 0), tok = pr / a.G;
-          cp_async16(sQ + (r >> 7) * kQBytes + (u >> 3) * kQChunk + swz128(r & 127, u & 7),
-                     q + (int64_t)(g.row0 + tok) * a.q_ld +
-                         (int64_t)(g.kvh * a.G + pr - tok * a.G) * HD + u * 8,
-                     valid);
+          cp_async16(dst + (r >> 7) * kQBytes + swz128(r & 127, u & 7), valid ? src : q, valid);
+          src += step * HD;
+          rem += step;
+          while (rem >= a.G) {
+            rem -= a.G;
+            src += a.q_ld - (int64_t)a.G * HD;
+          }
         }
         cp_async_wait_all();
         fence_proxy_async();
@@ -466,9 +484,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (po) {
           if (l != 0.f) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(po + c + e) =
-                  make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+            for (int e = 0; e < 32; e += 8) st_v8(po + c + e, ov + e);
           }
           continue;
         }
@@ -487,9 +503,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         if (a.o32) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(a.o32 + at + e) =
-                make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+          for (int e = 0; e < 32; e += 8) st_v8(a.o32 + at + e, ov + e);
         } else {
           __nv_bfloat16* dst =
               static_cast<__nv_bfloat16*>(a.o) + (int64_t)orow * a.o_ld + head * HD + c;

@@ -209,6 +209,16 @@ class ParallelDrafter(nn.Module):
         else:
             x[:] = self.real_input(ids.to(dev), feats.to(dev))
         cu, slots, pos = cache.resize([h + (n + k - 1 if n else 0) for h, n in zip(before, news)])
+        kept = before
+        try:
+            x = self._layers_cached(cache, x, cu, slots, pos)
+            kept = [h + n for h, n in zip(before, news)]
+        finally:  # without the prediction slots; as it was, where the pass was refused
+            if kept != cache.lengths:
+                cache.resize(kept)
+        return x, first
+
+    def _layers_cached(self, cache, x, cu, slots, pos):
         nh, nkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
         for i, layer in enumerate(self.layers):
             at = layer.attn
@@ -216,7 +226,7 @@ class ParallelDrafter(nn.Module):
             q, key, v = (ops.linear(h, m.weight) for m in (at.q_proj, at.k_proj, at.v_proj))
             ops.rope_(q, nh, hd, pos, self.rope_theta)
             ops.rope_(key, nkv, hd, pos, self.rope_theta)
-            with torch.cuda.device(dev):
+            with torch.cuda.device(x.device):
                 ops.cache_append(key, v, slots, cache.k[i], cache.v[i])
                 if cache.shared:
                     o, _ = ops.attn_paged_shared(q, cache.k[i], cache.v[i], cache.table,
@@ -228,10 +238,8 @@ class ParallelDrafter(nn.Module):
             w = torch.cat([layer.mlp.gate_proj.weight, layer.mlp.up_proj.weight], dim=0)
             act = ops.swiglu_fwd(ops.linear(h, w), self.intermediate)
             x = ops.linear(act, layer.mlp.down_proj.weight, residual=x)
-        if k > 1:
-            cache.resize([h + n for h, n in zip(before, news)])
         fnorm = self._final_norm[0]
-        return ops.rmsnorm_fwd(x, fnorm.weight, fnorm.eps)[0], first
+        return ops.rmsnorm_fwd(x, fnorm.weight, fnorm.eps)[0]
 
     @torch.no_grad()
     def draft_logits_cached(self, cache, ids: torch.Tensor, feats: torch.Tensor,
