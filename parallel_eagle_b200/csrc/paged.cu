@@ -64,7 +64,7 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
   bool joined = false;
 
   start_next_kernel();
-  Sched<Mt, kTK, kTK> w(a);
+  Sched<Mt, kTK, kTK, 3 * kTK> w(a);
   w.init(scratch);
   if (tid == 0) a.open[blockIdx.x].parts = 0;
   while (w.next()) {

@@ -14,6 +14,8 @@
 // the entity's first piece records how many there are; the combine kernel joins them in
 // piece order, so results do not depend on timing.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 
 namespace pe {
@@ -89,8 +91,9 @@ struct Seg {
 };
 
 // Mt: packed rows per tile.  TK: keys per tile.  kOver: what a segment's start and end cost
-// on top of its keys, in keys (Q rows in, result rows out, the pipeline's filling).
-template <int Mt, int TK, int kOver>
+// on top of its keys, in keys (Q rows in, result rows out, the pipeline's filling).  kLeast:
+// keys below which no block's piece goes (a small call ends sooner on fewer blocks).
+template <int Mt, int TK, int kOver, int kLeast>
 struct Sched {
   const Args& a;
   int64_t total, per, pos, end;  // cost units; this block's piece is [pos, end)
@@ -161,8 +164,8 @@ struct Sched {
       sum += scratch[w];
     }
     total = sum;
-    // an equal share each, but no piece below two key tiles' work
-    per = max(div_pos(total + gridDim.x - 1, gridDim.x), (int64_t)3 * TK * a.G);
+    // an equal share each, but none too small
+    per = max(div_pos(total + gridDim.x - 1, gridDim.x), (int64_t)kLeast * a.G);
     pos = min(total, (int64_t)blockIdx.x * per);
     end = min(total, pos + per);
     // the thread whose requests hold pos finds the request
@@ -277,6 +280,20 @@ __device__ __forceinline__ void start_next_kernel() {
 }
 __device__ __forceinline__ void wait_kernel_before() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Let kernel K use `bytes` of dynamic shared memory (always the same number), once per device:
+// the runtime's call costs as much as a quarter of a launch.
+template <auto K>
+inline int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int dev = 0;
+  PE_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return PE_OK;
+  PE_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return PE_OK;
 }
 
 // launch, optionally as a dependent of the kernel before it in the stream

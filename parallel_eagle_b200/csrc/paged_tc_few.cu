@@ -186,7 +186,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     tmem_alloc(&sm.tmem, F::kTmem);
     tmem_relinquish();
   }
-  Sched<N, kTile, kOver> w(a);
+  Sched<N, kTile, kOver, 2 * kTile> w(a);
   w.init(sm.scratch);
   tc_fence_before();
   __syncthreads();
@@ -622,7 +622,8 @@ int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
   if (rc) return rc;
   auto kern = paged_few_kernel<N, HDC>;
   constexpr int smem = (int)Few<N, HDC>::kSmem;
-  PE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int rcs = allow_smem<paged_few_kernel<N, HDC>>(smem);
+  if (rcs) return rcs;
   return launch_kernel(kern, dim3((unsigned)blocks), Few<N, HDC>::kThreads, smem, st, dependent, tk,
                        tv, a, box);
 }

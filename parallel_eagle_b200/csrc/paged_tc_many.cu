@@ -120,7 +120,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tmem_alloc(&sm.tmem, 512);
     tmem_relinquish();
   }
-  Sched<kRows, kTile, kOver> w(a);
+  Sched<kRows, kTile, kOver, 4 * kTile> w(a);
   w.init(sm.scratch);
   tc_fence_before();
   __syncthreads();
@@ -549,7 +549,8 @@ int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
   auto kern = paged_many_kernel<HDC>;
   constexpr int smem = (int)smem_bytes<HDC>();
   static_assert(smem <= 227 * 1024, "shared memory");
-  PE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int rcs = allow_smem<paged_many_kernel<HDC>>(smem);
+  if (rcs) return rcs;
   const int o_vec = (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 && a.o_ld % 8 == 0;
   return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, tk, tv, a, box,
                        o_vec);

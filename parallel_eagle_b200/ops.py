@@ -611,9 +611,11 @@ def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
     table_ld = _table_stride("attn_paged", table, batch)
     dev = q.device
     if o is None:
-        o = torch.empty(T, cols, dtype=dtype, device=dev)
+        o, o_ld = torch.empty(T, cols, dtype=dtype, device=dev), cols
     elif o.shape != q.shape or o.dtype is not dtype or o.device != dev:
         raise L.PeError(f"attn_paged: o must be like q, got {tuple(o.shape)} {o.dtype}")
+    else:
+        o_ld = _row_stride(o)
     if lse is None:
         lse = torch.empty(heads, T, dtype=torch.float32, device=dev)
     elif (lse.shape != (heads, T) or lse.dtype is not torch.float32 or not lse.is_contiguous()
@@ -627,7 +629,7 @@ def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
     rc = _lib().pe_attn_paged(
         code, batch, T, heads, hkv, hd, q.data_ptr(), _row_stride(q), k_cache.data_ptr(),
         v_cache.data_ptr(), pages, page, table.data_ptr(), table_ld, table.shape[1],
-        lens.data_ptr(), cu.data_ptr(), shared, o.data_ptr(), _row_stride(o), lse.data_ptr(),
+        lens.data_ptr(), cu.data_ptr(), shared, o.data_ptr(), o_ld, lse.data_ptr(),
         ws.data_ptr(), nbytes, algo, status_word(dev).data_ptr(),
         torch._C._cuda_getCurrentRawStream(idx),
     )
