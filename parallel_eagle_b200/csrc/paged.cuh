@@ -141,6 +141,36 @@ struct Sched {
     return (int64_t)a.Hkv * head_cost(r);
   }
 
+  // The piece of a block whose one warp walks the line, by that warp alone: no barrier, and
+  // the lengths' way from memory overlaps the block's other preparations.  (A lane looks at
+  // every 32nd part of the requests; from some hundred on the whole block is quicker.)
+  static constexpr int kWarpRequests = 128;
+  __device__ __forceinline__ void init_warp() {
+    const int n = requests(), lane = threadIdx.x & 31;
+    const int chunk = (n + 31) / 32, i0 = min(n, lane * chunk), i1 = min(n, i0 + chunk);
+    int64_t mine = 0;
+    for (int i = i0; i < i1; ++i) mine += req_cost(request(i));
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    total = __shfl_sync(0xffffffffu, inc, 31);
+    per = max(div_pos(total + gridDim.x - 1, gridDim.x), (int64_t)kLeast * a.G);
+    pos = min(total, (int64_t)blockIdx.x * per);
+    end = min(total, pos + per);
+    seg = 0;
+    b = 0;
+    base = inc - mine;
+    if (pos >= end) return;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, pos < inc)) - 1;
+    b = __shfl_sync(0xffffffffu, i0, owner);
+    base = __shfl_sync(0xffffffffu, base, owner);
+    rq = request(b);
+    // (next() steps over the owner's requests before pos)
+  }
+
   // all threads of the block; scratch: one int64 per warp plus 4
   __device__ __forceinline__ void init(int64_t* scratch) {
     const int n = requests(), tid = threadIdx.x, nthr = blockDim.x;

@@ -187,7 +187,10 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     tmem_relinquish();
   }
   Sched<N, kTile, kOver, 2 * kTile> w(a);
-  w.init(sm.scratch);
+  if (w.requests() > w.kWarpRequests)
+    w.init(sm.scratch);
+  else if (warp == 2)
+    w.init_warp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

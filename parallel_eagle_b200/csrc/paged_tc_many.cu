@@ -121,7 +121,10 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     tmem_relinquish();
   }
   Sched<kRows, kTile, kOver, 4 * kTile> w(a);
-  w.init(sm.scratch);
+  if (w.requests() > w.kWarpRequests)
+    w.init(sm.scratch);
+  else if (warp == 2)
+    w.init_warp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -575,3 +575,13 @@ def test_refusals():
                      ((ln[:0], ln[:0], table[:0], free, ring, 16, 2), {})):
         with pytest.raises(L.PeError):
             ops.cache_plan(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_requests(dtype):
+    """Batches whose line of work a warp, or the whole block, looks through."""
+    for batch in (31, 33, 128, 129, 700):
+        lens = [(37 * i) % 90 for i in range(batch)]
+        news = [min(t, 1 + i % 3) if i % 11 else 0 for i, t in enumerate(lens)]
+        case = make(lens, news, 4, 2, 64, 16, dtype, seed=batch)
+        check(*case, 4, *attend(case))
