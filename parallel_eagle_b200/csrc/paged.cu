@@ -71,6 +71,7 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
     const int rows = w.tile_rows();
     const int rr = w.rt * Mt + r;  // this thread's packed row
     const bool valid = r < rows;
+    const bool active = (tid >> 5) * 4 < rows;  // some of this warp's four rows
     const int64_t lim = valid ? w.limit(rr) : 0;
     // start the copies of tile t (zeros behind the last key and outside the pool)
     auto fetch = [&](int t) {
@@ -129,6 +130,7 @@ paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncthreads();  // tile t is here, tile t - 1 is read
       if (t + 1 < w.t1) fetch(t + 1);
+      if (!active) continue;
       const T* sK = sKV + (t & 1) * 2 * kTK * ldk;
       const T* sV = sK + kTK * ldk;
       float s[4] = {0.f, 0.f, 0.f, 0.f};

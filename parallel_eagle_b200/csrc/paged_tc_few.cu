@@ -38,7 +38,7 @@ using namespace sm100;
 
 constexpr int kTile = 128;                    // keys per tile
 constexpr uint32_t kChunk = kTile * 128;      // 128 keys x 64 columns, 128-byte swizzled
-constexpr int kOver = 2 * kTile;              // a segment's start and end, in keys
+constexpr int kOver = 6 * kTile;              // a segment's start and end, in keys
 constexpr float kRaise = 8.f;                 // log2 of what a score may pass the bound by
 
 template <int N, int HDC>

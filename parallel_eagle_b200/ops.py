@@ -39,7 +39,7 @@ def check_status(device: torch.device) -> None:
 
 
 def _lib():
-    return L.load()
+    return L._lib or L.load()
 
 
 def _row_stride(t: torch.Tensor) -> int:
