@@ -139,7 +139,7 @@ __device__ __forceinline__ void lane_sums(float (&v)[N], int lane) {
 template <int N, int HDC>
 __global__ void __launch_bounds__(Few<N, HDC>::kThreads, 1)
 paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                 const __grid_constant__ Args a, int box) {
+                 const __grid_constant__ Args a, int shift) {
   using F = Few<N, HDC>;
   constexpr int ST = F::kStages, QB = F::kQBufs, NG = F::kGroups, CW = F::kCols;
   constexpr int HD = 64 * HDC;
@@ -208,27 +208,31 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA ----
-    const int per_chunk = kTile / box, boxes = per_chunk * HDC;  // of a chunk, of a tile
-    const int at = lane % per_chunk, ch = lane / per_chunk;      // this lane's box
-    const int total_rows = (int)(a.num_pages * a.Hkv * a.page);
+    const int per_chunk = kTile >> shift, boxes = per_chunk * HDC;  // of a chunk, of a tile
+    const int box = 1 << shift;                                     // keys of a box
+    const int at = lane % per_chunk, ch = lane / per_chunk;         // this lane's box
+    const int total_rows = (int)(a.num_pages * a.Hkv * a.page), kbeg = (int)a.kbeg;
     bool ok = true;
     int i = 0;
     uint32_t st = 0, ph = 0;
     Seg g;
+    PageWalk pw;
     for (int s = 0; ok; ++s) {
       ok = take(s, g);
       if (!ok || g.end) break;
+      const int kend = (int)g.kend;
+      if (g.t0 < g.t1)
+        pw.start(g.pages, (kbeg + g.t0 * kTile) / a.page, (kend + a.page - 1) / a.page);
       for (int t = g.t0; t < g.t1; ++t, ++i) {
-        const int64_t k0 = a.kbeg + (int64_t)t * kTile;
-        const int live = min(per_chunk, (int)((g.kend - k0 + box - 1) / box));
+        const int k0 = kbeg + t * kTile;
+        const int live = min(per_chunk, (kend - k0 + box - 1) >> shift);
         const bool mine = lane < boxes && at < live;
-        int row = total_rows;  // (reads as zeros)
-        if (mine) {
-          const int64_t key = k0 + at * box, pi = div_pos(key, a.page);
-          const int id = g.pages[pi];
-          if (id >= 0 && id < a.num_pages)
-            row = (int)(((int64_t)id * a.Hkv + g.kvh) * a.page + (key - pi * a.page));
-        }
+        const int key = k0 + (mine ? at << shift : 0), pi = (int)((uint32_t)key / (uint32_t)a.page);
+        pw.advance((int)((uint32_t)k0 / (uint32_t)a.page));
+        const int id = pw.entry(pi, (int)((uint32_t)(k0 + kTile - 1) / (uint32_t)a.page));
+        // (an entry outside the pool reads as zeros)
+        const int row = id >= 0 && id < a.num_pages
+                            ? (id * a.Hkv + g.kvh) * a.page + (key - pi * a.page) : total_rows;
         const uint32_t off = st * F::kTileBytes + ch * kChunk + at * box * 128;
         const uint32_t bytes = (uint32_t)live * HDC * box * 128;
         ok = mbar_wait(&sm.k_empty[st], ph ^ 1u, status, 402);
@@ -616,19 +620,19 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 
 template <int N, int HDC>
 int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
-  int box = kTile;
-  while (a.page % box) box >>= 1;  // (pages are multiples of 16)
+  int shift = 7;  // boxes of up to a tile's keys that divide a page (a multiple of 16)
+  while (a.page % (1 << shift)) --shift;
   CUtensorMap tk, tv;
   const uint64_t rows = (uint64_t)a.num_pages * a.Hkv * a.page;
-  int rc = make_tmap_2d(&tk, a.kc, 64 * HDC, rows, 128 * HDC, 64, (uint32_t)box);
-  if (!rc) rc = make_tmap_2d(&tv, a.vc, 64 * HDC, rows, 128 * HDC, 64, (uint32_t)box);
+  int rc = make_tmap_2d(&tk, a.kc, 64 * HDC, rows, 128 * HDC, 64, 1u << shift);
+  if (!rc) rc = make_tmap_2d(&tv, a.vc, 64 * HDC, rows, 128 * HDC, 64, 1u << shift);
   if (rc) return rc;
   auto kern = paged_few_kernel<N, HDC>;
   constexpr int smem = (int)Few<N, HDC>::kSmem;
   const int rcs = allow_smem<paged_few_kernel<N, HDC>>(smem);
   if (rcs) return rcs;
   return launch_kernel(kern, dim3((unsigned)blocks), Few<N, HDC>::kThreads, smem, st, dependent, tk,
-                       tv, a, box);
+                       tv, a, shift);
 }
 
 }  // namespace

@@ -76,7 +76,7 @@ __device__ __forceinline__ void cp_async_wait_all() {
 template <int HDC>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const __grid_constant__ Args a, int box, int o_vec) {
+                  const __grid_constant__ Args a, int shift, int o_vec) {
   constexpr int HD = 64 * HDC;
   constexpr uint32_t kTileBytes = HDC * kChunk, kQBytes = HDC * kQChunk;
   extern __shared__ uint8_t smem_raw[];
@@ -148,27 +148,31 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (warp < 4) {
     if (warp == 0) {
       // ---------------------------------------------------------------- TMA ----
-      const int per_chunk = kTile / box, boxes = per_chunk * HDC;
-      const int at = lane % per_chunk, ch = lane / per_chunk;
-      const int total_rows = (int)(a.num_pages * a.Hkv * a.page);
+      const int per_chunk = kTile >> shift, boxes = per_chunk * HDC;  // of a chunk, of a tile
+      const int box = 1 << shift;                                     // keys of a box
+      const int at = lane % per_chunk, ch = lane / per_chunk;         // this lane's box
+      const int total_rows = (int)(a.num_pages * a.Hkv * a.page), kbeg = (int)a.kbeg;
       bool ok = true;
       int i = 0;
       uint32_t st = 0, ph = 0;
       Seg g;
+      PageWalk pw;
       for (int s = 0; ok; ++s) {
         ok = take(s, g);
         if (!ok || g.end) break;
+        const int kend = (int)g.kend;
+        if (g.t0 < g.t1)
+          pw.start(g.pages, (kbeg + g.t0 * kTile) / a.page, (kend + a.page - 1) / a.page);
         for (int t = g.t0; t < g.t1; ++t, ++i) {
-          const int64_t k0 = a.kbeg + (int64_t)t * kTile;
-          const int live = min(per_chunk, (int)((g.kend - k0 + box - 1) / box));
+          const int k0 = kbeg + t * kTile;
+          const int live = min(per_chunk, (kend - k0 + box - 1) >> shift);
           const bool mine = lane < boxes && at < live;
-          int row = total_rows;  // (reads as zeros)
-          if (mine) {
-            const int64_t key = k0 + at * box, pi = div_pos(key, a.page);
-            const int id = g.pages[pi];
-            if (id >= 0 && id < a.num_pages)
-              row = (int)(((int64_t)id * a.Hkv + g.kvh) * a.page + (key - pi * a.page));
-          }
+          const int key = k0 + (mine ? at << shift : 0), pi = (int)((uint32_t)key / (uint32_t)a.page);
+          pw.advance((int)((uint32_t)k0 / (uint32_t)a.page));
+          const int id = pw.entry(pi, (int)((uint32_t)(k0 + kTile - 1) / (uint32_t)a.page));
+          // (an entry outside the pool reads as zeros)
+          const int row = id >= 0 && id < a.num_pages
+                              ? (id * a.Hkv + g.kvh) * a.page + (key - pi * a.page) : total_rows;
           const uint32_t bytes = (uint32_t)live * HDC * box * 128;
           const uint32_t off = st * kTileBytes + ch * kChunk + at * box * 128;
           ok = mbar_wait(&sm.k_empty[st], ph ^ 1u, status, 422);
@@ -542,12 +546,12 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 
 template <int HDC>
 int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
-  int box = kTile;
-  while (a.page % box) box >>= 1;  // (pages are multiples of 16)
+  int shift = 6;  // boxes of up to a tile's keys that divide a page (a multiple of 16)
+  while (a.page % (1 << shift)) --shift;
   CUtensorMap tk, tv;
   const uint64_t rows = (uint64_t)a.num_pages * a.Hkv * a.page;
-  int rc = make_tmap_2d(&tk, a.kc, 64 * HDC, rows, 128 * HDC, 64, (uint32_t)box);
-  if (!rc) rc = make_tmap_2d(&tv, a.vc, 64 * HDC, rows, 128 * HDC, 64, (uint32_t)box);
+  int rc = make_tmap_2d(&tk, a.kc, 64 * HDC, rows, 128 * HDC, 64, 1u << shift);
+  if (!rc) rc = make_tmap_2d(&tv, a.vc, 64 * HDC, rows, 128 * HDC, 64, 1u << shift);
   if (rc) return rc;
   auto kern = paged_many_kernel<HDC>;
   constexpr int smem = (int)smem_bytes<HDC>();
@@ -555,7 +559,7 @@ int launch(const Args& a, int blocks, bool dependent, cudaStream_t st) {
   const int rcs = allow_smem<paged_many_kernel<HDC>>(smem);
   if (rcs) return rcs;
   const int o_vec = (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0 && a.o_ld % 8 == 0;
-  return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, tk, tv, a, box,
+  return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, tk, tv, a, shift,
                        o_vec);
 }
 
