@@ -364,7 +364,7 @@ int pe_wait_probe(uint64_t limit_ns, int32_t* status, int32_t* waited_out, void*
  * pages given back in a call are not taken in it.  The first `shared` keys (whole pages)
  * of every request belong to a shared prefix whose pages are neither taken nor given back.
  *   granted[b]  new_lens[b], or lens[b] when the request is refused: lengths that are
- *               negative or beyond the table, growth once the pages run out (all later
+ *               negative, below `shared` or beyond the table, growth once the pages run out (all later
  *               growth with it), pages given back that the ring has no room for
  *   cu[B + 1]   first new row of each request (max(0, new_lens - lens) rows each)
  *   slots/pos   per new row, `rows` of them: slot (page * page_size + offset; -1 for a

@@ -84,7 +84,8 @@ plan_kernel(int B, int64_t width, int N, int page, int64_t rows, int sp,
     if (b < B) {
       const int from = lens[b], to = want[b];
       const int64_t u = ((int64_t)from + page - 1) / page, n = ((int64_t)to + page - 1) / page;
-      const bool fits = from >= 0 && to >= 0 && u <= width && n <= width;
+      const int64_t least = (int64_t)sp * page;  // (rows below would land in the shared pages)
+      const bool fits = from >= least && to >= least && u <= width && n <= width;
       const int used = max((int)u, sp), need = max((int)n, sp);
       s_from[b] = from;
       s_used[b] = fits ? used : -1;

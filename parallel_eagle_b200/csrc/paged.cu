@@ -479,5 +479,8 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
   }
   const Phase p = tc ? tc_phase(ceil_div(T * a.G, B)) : simt_phase(dtype, hd);
   carve(a, p, ws);
-  return run_phase(dtype, p, a, shared > 0, st);
+  // The requests' own keys start while the prefix ends, unless it takes long (here: some 10
+  // ms): nothing is gained then, and a block's bounded waits would run while it waits.
+  const bool brief = 4.0 * (double)T * Hq * hd * (double)shared < 1e13;
+  return run_phase(dtype, p, a, shared > 0 && brief, st);
 }

@@ -225,7 +225,8 @@ struct Sched {
     int64_t rc = req_cost(rq);
     while (pos >= base + rc) {  // (requests without rows cost nothing)
       base += rc;
-      rq = request(++b);
+      if (++b >= requests()) return false;  // (row offsets that make no sense)
+      rq = request(b);
       rc = req_cost(rq);
     }
     const int64_t per_head = head_cost(rq);

@@ -511,7 +511,7 @@ def cache_plan(lens, new_lens, table, free, ring, page: int, rows: int, *, share
     request was refused), the first new row of each request (int32 ``[B + 1]``), each new
     row's cache slot and position (int64 ``[rows]``) and the ring after the call, whose last
     entry counts refused requests.  The first ``shared`` keys (whole pages) of all requests
-    belong to a shared prefix and are left alone."""
+    belong to a shared prefix and are left alone; a request is never shorter."""
     if ring_out is None:
         ring_out = torch.empty_like(ring)
     idx = _one_device(lens, new_lens, table, free, ring, ring_out)
@@ -525,6 +525,7 @@ def cache_plan(lens, new_lens, table, free, ring, page: int, rows: int, *, share
         if t.dtype is not torch.int64 or t.dim() != 1 or t.numel() != 3 or not t.is_contiguous():
             _refuse_ints("cache_plan: ring and ring_out", t, "3", torch.int64)
     table_ld = _table_stride("cache_plan", table, batch)
+    page, rows, shared = int(page), int(rows), int(shared)
     if rows < 0:
         raise L.PeError(f"cache_plan: {rows} new rows")
     dev = lens.device
@@ -586,11 +587,11 @@ def attn_paged_shared(q, k_cache, v_cache, table, lens, cu, shared: int, o=None,
     prefix (``lens[b] - n_b >= shared``)."""
     if shared < 0:
         raise L.PeError(f"attn_paged_shared: {shared} shared keys")
-    return _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo)
+    return _attn_paged(q, k_cache, v_cache, table, lens, cu, int(shared), o, lse, algo)
 
 
 @functools.lru_cache(maxsize=1024)
-def _attn_paged_bytes(*sizes: int) -> int:
+def _attn_paged_bytes(device: int, *sizes: int) -> int:
     return int(_lib().pe_attn_paged_workspace(*sizes))
 
 
@@ -622,7 +623,7 @@ def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
           or lse.device != dev):
         raise L.PeError(f"attn_paged: lse must be contiguous float32 [{heads}, {T}]")
     code = L.dtype_code(dtype)
-    nbytes = _attn_paged_bytes(code, batch, T, heads, hkv, hd, shared)
+    nbytes = _attn_paged_bytes(idx, code, batch, T, heads, hkv, hd, shared)
     # the call's own scratch, from torch's stream-ordered allocator: calls on other streams
     # and captured graphs never share it
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -49,7 +49,7 @@ def plan_reference(lens, want, table, free, head, tail, page, rows, shared=0):
     granted, cu, slots, pos = [], [0], [], []
     pushes, broke_grow, broke_drop = [], False, False
     for b, (a, z) in enumerate(zip(lens, want)):
-        fits = a >= 0 and z >= 0 and -(-a // page) <= width and -(-z // page) <= width
+        fits = min(a, z) >= shared and -(-a // page) <= width and -(-z // page) <= width
         used, need = max(-(-a // page), sp), max(-(-z // page), sp)
         ok = fits
         if fits and need > used:
@@ -135,6 +135,17 @@ def test_plan_with_shared_prefix_leaves_its_pages():
     case = _plan_case(50, 16, 12, 900, seed=4, head=2, shared=48)
     got = run_plan(*case)
     assert int(got[4][2]) == 0
+
+
+def test_plan_refuses_lengths_below_the_shared_prefix():
+    """Rows below it would land in the pages that all requests read."""
+    table = [[8, 9, 0], [8, 9, 1], [8, 9, 2]]
+    free = [3, 4, 5, -1, -1, -1, -1, -1, -1, -1]
+    # (request 0 outgrows the table's three pages)
+    got = run_plan([32, 10, 40], [50, 40, 16], table, free, 0, 3, 16, 18 + 30, shared=32)
+    assert got[0].tolist() == [32, 10, 40] and int(got[4][2]) == 3
+    got = run_plan([32, 10, 40], [47, 40, 16], table, free, 0, 3, 16, 15 + 30, shared=32)
+    assert got[0].tolist() == [47, 10, 40] and int(got[4][2]) == 2
 
 
 def test_plan_refuses_lengths_and_pads_rows():
@@ -347,6 +358,26 @@ def test_attention_long_ragged(dtype, page):
         check(*case, 28, *attend(case))
     case = make([9000], [6], 14, 2, 64, page, dtype, seed=page + 1)
     check(*case, 14, *attend(case))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_one_long_request(dtype, hd):
+    """One request over all blocks (its pieces joined), single tokens and drafts."""
+    for total, n in ((70001, 1), (33333, 5), (20000, 40)):
+        case = make([total], [n], 4, 1, hd, 128, dtype, seed=n)
+        check(*case, 4, *attend(case))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_row_offsets_that_make_no_sense_stay_in_bounds(dtype):
+    """Offsets behind the rows, or running backwards: nothing outside the rows is touched."""
+    q, kc, vc, table, lens, _ = make([90, 60, 30], [4, 4, 4], 4, 2, 64, 16, dtype)
+    for cu in ([0, 400, 800, 1200], [5, 2, 9, 1], [-7, 3, 3, 2**31 - 1], [0, 4, 8, 12]):
+        out = torch.full((q.shape[0] + 2, q.shape[1]), 7.0, dtype=dtype, device=DEV)
+        o, _ = ops.attn_paged(q, kc, vc, table, _i32(lens), _i32(cu), o=out[1:-1])
+        assert (out[0] == 7).all() and (out[-1] == 7).all()
+    check(q, kc, vc, table, lens, cu, 4, *attend((q, kc, vc, table, lens, cu)))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
