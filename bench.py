@@ -918,10 +918,13 @@ def run_draft(args):
     config-2 dims, one context of ``--n`` (default 2048) confirmed tokens, k = 5.
     Times, with CUDA events on the launching stream, ``draft_logits`` (one forward
     over p + k - 1 slots + the LM head on k rows), ``propose_tree`` (k 5, top_k 4,
-    max_nodes 20; includes the host beam and its device reads) and the sequential
-    baseline ``draft_logits_sequential``; the CPU oracle's ``draft_logits`` on a
+    max_nodes 20; includes the host beam and its device reads), the sequential
+    baseline ``draft_logits_sequential``, and ``draft_logits_cached`` for one and for
+    eight requests that hold the context in a key/value cache and get 3 new tokens
+    (whose rows are taken back after each call); the CPU oracle's ``draft_logits`` on a
     bounded context is reported beside it."""
     from parallel_eagle_b200 import decode, ops
+    from parallel_eagle_b200.cache import DraftCache
 
     dev = torch.device("cuda", 0)
     torch.cuda.set_device(dev)
@@ -937,10 +940,26 @@ def run_draft(args):
         "propose_tree": lambda: decode.propose_tree(d, ids, feats, k, 4, 20),
         "draft_logits_sequential": lambda: d.draft_logits_sequential(ids, feats, k),
     }
+    tokens = {}
+    new = min(3, p - 1)
+    for batch in (1, 8):
+        cache = DraftCache(d, batch, pages=batch * (-(-(p + k) // 64) + 1))
+        for b in range(batch):  # the context, one request at a time
+            news = [p - new if r == b else 0 for r in range(batch)]
+            d.draft_logits_cached(cache, ids[:p - new], feats[:p - new], news, k)
+        more = ids[p - new:].repeat(batch), feats[p - new:].repeat(batch, 1)
+
+        def cached(cache=cache, more=more, batch=batch):
+            d.draft_logits_cached(cache, *more, [new] * batch, k)
+            cache.resize([p - new] * batch)
+
+        name = f"draft_logits_cached_{batch}"
+        runs[name], tokens[name] = cached, batch * k
     out = {}
     for name, fn in runs.items():
         ms = time_case(fn, args.steps, warmup=args.warmup)
-        out[name] = {"ms": round(ms, 3), "draft_tokens_per_s": round(k / (ms / 1e3), 1)}
+        out[name] = {"ms": round(ms, 3),
+                     "draft_tokens_per_s": round(tokens.get(name, k) / (ms / 1e3), 1)}
     ops.check_status(dev)
     line = {"metric": "draft latency (k=5 tokens after a confirmed context)", "unit": "ms",
             "higher_is_better": False, "dtype": "bf16", "data": "synthetic",

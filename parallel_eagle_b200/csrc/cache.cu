@@ -25,8 +25,8 @@ namespace {
 // finding an index's request by bisection in shared memory.  A row's page comes straight
 // from the ring when this call is the one that takes it, so no block reads what another
 // writes and one launch does it all.  A thread describes two rows (one bisection, 16-byte
-// stores).  Bound by launch latency up to some 100K rows, by the 16 bytes written per row
-// above.
+// stores).  Bound by latency: a scan, then per row a bisection and one dependent read of the
+// ring or the table.  Measured: 8 drafts 5.2 us, 512 requests with 811K new rows 14 us.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanBatch = 8192;  // requests whose scan fits the block's shared memory
 
@@ -196,7 +196,8 @@ plan_kernel(int B, int64_t width, int N, int page, int64_t rows, int sp,
 // Row t of k / v -> its slot in the cache: per head a contiguous run of hd elements.  A
 // copy, bound by HBM: one read and one write of each row.  A thread moves kItems pieces
 // of K and of V (16 bytes each when rows and cache allow it), with all of its loads
-// issued before the first store.
+// issued before the first store.  Measured: 16411 rows of 8 x 128 bf16 23.4 us, 5.75 TB/s
+// (0.89 of a plain copy); 48 rows 3.4 us.
 constexpr int kAppendThreads = 256;
 constexpr int kItems = 4;
 

@@ -19,7 +19,9 @@ namespace {
 // threads share a row's scores, statistics and output columns.  It serves fp32 (whose
 // products the tensor cores would round) and what the tensor-core kernels do not take.
 // Bound by shared-memory reads: a key's element is read once per 4 rows of a warp for the
-// scores and once for the output.
+// scores and once for the output.  Measured: 16 requests of 1..5 rows, 17K keys in all, 4/2
+// heads of 64, fp32: 25.5 us with the join, of which half is a block's start, its one or two
+// results and the join.
 constexpr int kThreads = 128;
 constexpr int kSimtRows = 16;
 constexpr int kTK = 32;

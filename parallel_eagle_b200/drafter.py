@@ -235,8 +235,10 @@ class ParallelDrafter(nn.Module):
                     o, _ = ops.attn_paged(q, cache.k[i], cache.v[i], cache.table, cache.lens, cu)
             x = ops.linear(o, at.o_proj.weight, residual=x)
             h, _ = ops.rmsnorm_fwd(x, layer.post_norm.weight, layer.post_norm.eps)
-            w = torch.cat([layer.mlp.gate_proj.weight, layer.mlp.up_proj.weight], dim=0)
-            act = ops.swiglu_fwd(ops.linear(h, w), self.intermediate)
+            gu = torch.empty(x.shape[0], 2 * self.intermediate, dtype=x.dtype, device=x.device)
+            ops.linear(h, layer.mlp.gate_proj.weight, out=gu[:, : self.intermediate])
+            ops.linear(h, layer.mlp.up_proj.weight, out=gu[:, self.intermediate :])
+            act = ops.swiglu_fwd(gu, self.intermediate)
             x = ops.linear(act, layer.mlp.down_proj.weight, residual=x)
         fnorm = self._final_norm[0]
         return ops.rmsnorm_fwd(x, fnorm.weight, fnorm.eps)[0]
