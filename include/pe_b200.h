@@ -390,14 +390,17 @@ int pe_cache_append(int dtype, int64_t rows, int Hkv, int hd, const void* k, int
  * gives o = 0, lse = -inf; rows behind cu[B] are left as they were.  lse: fp32 [Hq, T],
  * natural log.  Head sizes 1..256, Hq / Hkv <= 256, pages of a multiple of 16 keys.
  *
- * shared > 0 (whole pages): the first `shared` keys of every request are those of table row
- * 0; they are read once for all rows, and the requests' own keys joined to them.  Every
- * request with rows must then hold the prefix: lens[b] - n_b >= shared.
+ * shared > 0 (whole pages): the first `shared` keys of all requests are the same pages, in
+ * every row of the block table.  They are read once for all rows, and the requests' own keys
+ * joined to them -- where that is faster, or always with algo bit PE_PAGED_PREFIX_ONCE; a
+ * short prefix of few requests is read by each from L2.  Every request with rows must hold
+ * the prefix: lens[b] - n_b >= shared.
  *
  * What a cache holds behind a request's keys does not matter (NaN included); keys below
  * lens[b] are finite, or the rows of the tile that masks them may turn NaN too.  Block table
  * entries outside the pool read as zero keys and values.  workspace:
  * pe_attn_paged_workspace bytes, 256-byte aligned, for this call alone while it runs. */
+#define PE_PAGED_PREFIX_ONCE 0x100
 size_t pe_attn_paged_workspace(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd,
                                int64_t shared);
 int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, int hd, const void* q,

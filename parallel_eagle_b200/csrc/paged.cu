@@ -364,6 +364,21 @@ bool tc_operands(const Args& a) {
          a.num_pages * a.Hkv * a.page < (1ll << 31) - 256;
 }
 
+// Whether the requests read their common prefix each for itself.  Its pages then come from
+// L2 after the first time, and a prefix of its own costs two launches, an fp32 result and a
+// second start of the copies, 25 to 40 us.  Device time of (each for itself, once) in us,
+// by B * prefix keys * KV heads:
+//   bf16, 28/4 heads of 128, 1 row:   131K 20, 43   524K 36, 45   1.05M 56, 51   2.1M 102, 64
+//         5 rows:                     131K 27, 49   524K 51, 62   1.05M 84, 72   2.1M 155, 94
+//   bf16, 14/2 heads of 64, 5 rows:   131K 25, 45   524K 49, 55   1.05M 82, 65
+//   fp32, 4/2 heads of 64, 1 row:      66K 28, 39   131K 43, 45    262K 68, 55    524K 119, 63
+// With more rows a request than the few-row kernel takes, the prefix's rows of all requests
+// fill its tiles better than each request's.
+bool prefix_per_request(bool tc, int64_t B, int64_t rows, int64_t keys) {
+  if (tc && ceil_div(rows, B) > 64) return false;
+  return B * keys <= (tc ? 700000 : 160000);
+}
+
 int64_t al256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // bytes of one phase's partial results
@@ -415,6 +430,8 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
                              void* workspace, size_t workspace_bytes, int algo, int* status,
                              void* stream) {
   PE_CHECK_ARG(dtype == PE_F32 || dtype == PE_BF16, "attn_paged: unsupported dtype code %d", dtype);
+  const bool once = algo & PE_PAGED_PREFIX_ONCE;
+  algo &= ~PE_PAGED_PREFIX_ONCE;
   PE_CHECK_ARG(algo == PE_ALGO_AUTO || algo == PE_ALGO_SIMT || algo == PE_ALGO_TCGEN05,
                "attn_paged: unknown algorithm %d", algo);
   PE_CHECK_ARG(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 256,
@@ -458,6 +475,7 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
               "rows and pools below 2^31 keys x heads");
     return PE_ERR_UNSUPPORTED;
   }
+  if (shared > 0 && !once && prefix_per_request(tc, B, T * a.G, shared * Hkv)) shared = 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (shared > 0) {
     // the prefix once, all rows of all requests together, into fp32 rows

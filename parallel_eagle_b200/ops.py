@@ -582,9 +582,10 @@ def attn_paged(q, k_cache, v_cache, table, lens, cu, o=None, lse=None, algo=L.AL
 def attn_paged_shared(q, k_cache, v_cache, table, lens, cu, shared: int, o=None, lse=None,
                       algo=L.ALGO_AUTO):
     """:func:`attn_paged` for requests whose first ``shared`` keys (whole pages) are the same
-    pages -- samples or drafts forked from one prompt.  The prefix is taken from ``table[0]``
-    and read once for all rows; ``lens`` counts it.  Every request with rows holds the whole
-    prefix (``lens[b] - n_b >= shared``)."""
+    pages -- samples or drafts forked from one prompt -- in every row of ``table``.  The prefix
+    is read once for all rows unless it is so short that each request reads it faster for
+    itself (``algo | PAGED_PREFIX_ONCE``: always once); ``lens`` counts it.  Every request
+    with rows holds the whole prefix (``lens[b] - n_b >= shared``)."""
     if shared < 0:
         raise L.PeError(f"attn_paged_shared: {shared} shared keys")
     return _attn_paged(q, k_cache, v_cache, table, lens, cu, int(shared), o, lse, algo)

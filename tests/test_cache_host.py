@@ -57,7 +57,7 @@ def test_attention_validates():
                dict(hd=0), dict(hd=257), dict(B=0), dict(T=-1), dict(T=1 << 30), dict(page=8),
                dict(page=24), dict(pages=0), dict(width=0), dict(width=1 << 27, table_ld=1 << 27),
                dict(table_ld=3), dict(shared=-16), dict(shared=8), dict(shared=80), dict(q_ld=255),
-               dict(o_ld=128), dict(algo=7), dict(p=0)):
+               dict(o_ld=128), dict(algo=7), dict(algo=0x200), dict(p=0)):
         assert _attn(lib, **kw) == 1, kw
         assert b"attn_paged" in lib.pe_last_error()
     # a workspace that is missing, short or misaligned

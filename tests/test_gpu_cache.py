@@ -308,10 +308,11 @@ def check(q, kc, vc, table, lens, cu, hq, o, lse):
     assert (o[rows_dead] == 0).all()
 
 
-def attend(case, shared=0, algo=L.ALGO_AUTO, **kw):
+def attend(case, shared=0, algo=L.ALGO_AUTO, once=True, **kw):
     q, kc, vc, table, lens, cu = case
     if shared:
-        return ops.attn_paged_shared(q, kc, vc, table, _i32(lens), _i32(cu), shared, algo=algo, **kw)
+        return ops.attn_paged_shared(q, kc, vc, table, _i32(lens), _i32(cu), shared,
+                                     algo=algo | (L.PAGED_PREFIX_ONCE if once else 0), **kw)
     return ops.attn_paged(q, kc, vc, table, _i32(lens), _i32(cu), algo=algo, **kw)
 
 
@@ -390,6 +391,7 @@ def test_shared_prefix(dtype, heads, shared):
         lens = [shared + t for t in own]
         case = make(lens, news, hq, hkv, hd, 16, dtype, seed=shared, shared=shared)
         check(*case, hq, *attend(case, shared=shared))
+        check(*case, hq, *attend(case, shared=shared, once=False))  # by size
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -502,7 +504,8 @@ def test_capture_replay_and_side_stream(shared):
                                                      shared=shared)
         ops.cache_append(k, v, slots, kc, vc)
         if shared:
-            return ops.attn_paged_shared(q, kc, vc, tab, granted, c, shared)
+            return ops.attn_paged_shared(q, kc, vc, tab, granted, c, shared,
+                                         algo=L.PAGED_PREFIX_ONCE)
         return ops.attn_paged(q, kc, vc, tab, granted, c)
 
     s = torch.cuda.Stream()
@@ -581,7 +584,7 @@ def test_refusals():
         dict(cu=c[:1]), dict(cu=c.long()), dict(lens=ln.cpu()), dict(q=q[:1].expand(2, -1)),
         dict(k_cache=kc[:, :, :8].contiguous(), v_cache=vc[:, :, :8].contiguous()),  # page 8
         dict(o=torch.empty(2, 255, dtype=BF16, device=DEV)), dict(lse=torch.empty(2, 4, device=DEV)),
-        dict(algo=9),
+        dict(algo=9), dict(algo=0x200),
     ]
     for change in bad:
         with pytest.raises(L.PeError):
