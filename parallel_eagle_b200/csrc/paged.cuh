@@ -35,6 +35,7 @@ struct Args {
   int B, T, Hq, Hkv, hd, G;  // G = Hq / Hkv
   int64_t kbeg;           // first key (the shared prefix, when another launch does it)
   int all_rows;           // 1: one request of cu[B] rows that all see keys [kbeg, kmax)
+  int align;              // 1: pieces that cut every entity at the same places (all_rows)
   float scale_log2;       // log2(e) / sqrt(hd)
   void* o;                // result rows (the operand type), row stride o_ld
   int64_t o_ld;
@@ -158,6 +159,15 @@ struct Sched {
     }
     total = __shfl_sync(0xffffffffu, inc, 31);
     per = max(div_pos(total + gridDim.x - 1, gridDim.x), (int64_t)kLeast * a.G);
+    if (a.align) {
+      // A piece of a half entity's multiple (within a tenth of an equal share): blocks on the
+      // row tiles of one head then walk the same keys at the same time, and a key tile comes
+      // from HBM once for all of them.
+      const Req r = request(0);
+      const int64_t twice = r.R > 0 ? 2 * cost(r, 0) : 0, halves = div_pos(twice, per);
+      if (halves >= 2 && halves * per * 10 >= twice * 9)
+        per = div_pos(twice + halves - 1, halves);
+    }
     pos = min(total, (int64_t)blockIdx.x * per);
     end = min(total, pos + per);
     seg = 0;

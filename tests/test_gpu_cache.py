@@ -619,3 +619,11 @@ def test_many_requests(dtype):
         news = [min(t, 1 + i % 3) if i % 11 else 0 for i, t in enumerate(lens)]
         case = make(lens, news, 4, 2, 64, 16, dtype, seed=batch)
         check(*case, 4, *attend(case))
+
+
+def test_prefix_beyond_the_cache():
+    """A prefix of more than 64 MB, whose pieces are cut alike for all row tiles."""
+    shared = 20480
+    lens, news = [shared + 9 + 30 * i for i in range(20)], [5] * 20
+    case = make(lens, news, 40, 8, 128, 128, BF16, shared=shared)
+    check(*case, 40, *attend(case, shared=shared))
