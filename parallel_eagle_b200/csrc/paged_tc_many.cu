@@ -18,15 +18,16 @@
 // the next scores are there when a softmax ends, so both tiles' softmax run all the time;
 // with one S of 128 keys they took turns with their own products (3840 cycles per 128
 // keys, the tensor pipe half idle).  A row's maximum is only raised (and O rescaled) when
-// it grows by more than 2^8.  Every fourth pair of exponentials runs on the FMA pipe (0, 1/2,
-// 1/3 and 1/8 measured within 3 % of it).
+// it grows by more than 2^8.  The exponentials all run on the SFU: a share of them on the FMA
+// pipe was no faster (1/8, 1/4) or slower (1/2), and costs power.
 //
-// Measured: 320 rows a head over a prefix of 64K keys, 40/8 heads of 128, 460 us, 930
-// TFLOP/s (0.55 of the burst rate; the card ran at 1.6 GHz under its power cap); two prompts
-// of ~1000 rows over ~4K keys, 28/4 heads, 130 us.  Three things take about as long each:
-// without the softmax 390 us, without the products 380 us, copies and barriers alone 300 us.
-// With 64 keys a tile the scores read Q from shared memory once per 64 columns, which
-// bounds their products; 128 keys leave TMEM for one S a tile only (slower, above).
+// Measured: 1600 packed rows a KV head over a prefix of 64K keys, 40/8 heads of 128, 450 us
+// in single calls, 950 TFLOP/s (0.56 of the burst rate), and about 500 us when repeated
+// under the power cap; two prompts of ~1000 rows over ~4K keys, 28/4 heads, 135 us.  Three
+// things take about as long each: without the softmax 390 us, without the products 380 us,
+// copies and barriers alone 300 us.  With 64 keys a tile the scores read Q from shared
+// memory once per 64 columns, which bounds their products; 128 keys leave TMEM for one S a
+// tile only (slower, above).
 #include "paged.cuh"
 #include "sm100.cuh"
 
@@ -45,7 +46,6 @@ constexpr uint32_t kChunk = kTile * 128;      // 64 keys x 64 columns, 128-byte 
 constexpr uint32_t kQChunk = kHalf * 128;     // 128 rows x 64 columns
 constexpr int kOver = 4 * kTile;              // a segment's start and end, in keys
 constexpr float kRaise = 8.f;
-constexpr int kEmuEvery = 4;
 
 struct Small {
   Seg seg[2];
@@ -409,13 +409,7 @@ paged_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
             const float2 y = fma2(make_float2(x[c], x[c + 1]), sc, off);
-            float2 p;
-            if (kEmuEvery > 0 && (c / 2) % kEmuEvery == kEmuEvery - 1) {
-              p = exp2_poly2(y);
-            } else {
-              p.x = ex2_approx(y.x);
-              p.y = ex2_approx(y.y);
-            }
+            const float2 p = make_float2(ex2_approx(y.x), ex2_approx(y.y));
             rs[(c >> 1) & 3] = add2(rs[(c >> 1) & 3], p);
             pk[c / 2] = pack_bf16x2(p.x, p.y);
           }
