@@ -30,6 +30,10 @@ class DraftCache:
         if requests < 1 or pages < 1 or page < 16 or page % 16:
             raise ValueError(f"{requests} requests, {pages} pages of {page} keys: at least one "
                              "of each, pages a multiple of 16 keys")
+        if max_len is None:
+            max_len = pages * page
+        if max_len < 1:
+            raise ValueError(f"max_len must be positive, got {max_len}")
         dev, dtype = drafter.device, drafter.param_dtype
         if dev.type != "cuda":
             raise L.PeError("the draft cache is on CUDA only; move the drafter to a CUDA device")
@@ -37,7 +41,7 @@ class DraftCache:
         self.k = torch.zeros(shape, dtype=dtype, device=dev)
         self.v = torch.zeros(shape, dtype=dtype, device=dev)
         self.page, self.pages = page, pages
-        width = -(-(max_len or pages * page) // page)
+        width = -(-max_len // page)
         self.table = torch.zeros(requests, width, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=dev)
         self._free = torch.arange(pages, dtype=torch.int32, device=dev)

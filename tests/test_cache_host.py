@@ -105,3 +105,6 @@ def test_draft_cache_needs_a_gpu():
         DraftCache(d, 1, 4)
     with pytest.raises(ValueError, match="multiple of 16"):
         DraftCache(d, 1, 4, page=24)
+    for max_len in (0, -5):
+        with pytest.raises(ValueError, match="max_len"):
+            DraftCache(d, 1, 4, max_len=max_len)
