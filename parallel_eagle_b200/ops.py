@@ -528,10 +528,9 @@ def cache_plan(lens, new_lens, table, free, ring, page: int, rows: int, *, share
     page, rows, shared = int(page), int(rows), int(shared)
     if rows < 0:
         raise L.PeError(f"cache_plan: {rows} new rows")
-    dev = lens.device
     granted = torch.empty_like(lens)
-    cu = torch.empty(batch + 1, dtype=torch.int32, device=dev)
-    slots = torch.empty(rows, dtype=torch.int64, device=dev)
+    cu = lens.new_empty(batch + 1)
+    slots = ring.new_empty(rows)
     pos = torch.empty_like(slots)
     rc = _lib().pe_cache_plan(
         batch, table.shape[1], free.numel(), page, rows, shared, lens.data_ptr(),
@@ -593,7 +592,7 @@ def attn_paged_shared(q, k_cache, v_cache, table, lens, cu, shared: int, o=None,
 
 @functools.lru_cache(maxsize=1024)
 def _attn_paged_bytes(device: int, *sizes: int) -> int:
-    return int(_lib().pe_attn_paged_workspace(*sizes))
+    return int(_lib().pe_attn_paged_workspace(*sizes))  # (a multiple of 256)
 
 
 def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
@@ -613,13 +612,13 @@ def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
     table_ld = _table_stride("attn_paged", table, batch)
     dev = q.device
     if o is None:
-        o, o_ld = torch.empty(T, cols, dtype=dtype, device=dev), cols
+        o, o_ld = q.new_empty(T, cols), cols
     elif o.shape != q.shape or o.dtype is not dtype or o.device != dev:
         raise L.PeError(f"attn_paged: o must be like q, got {tuple(o.shape)} {o.dtype}")
     else:
         o_ld = _row_stride(o)
     if lse is None:
-        lse = torch.empty(heads, T, dtype=torch.float32, device=dev)
+        lse = q.new_empty(heads, T, dtype=torch.float32)
     elif (lse.shape != (heads, T) or lse.dtype is not torch.float32 or not lse.is_contiguous()
           or lse.device != dev):
         raise L.PeError(f"attn_paged: lse must be contiguous float32 [{heads}, {T}]")
@@ -627,7 +626,7 @@ def _attn_paged(q, k_cache, v_cache, table, lens, cu, shared, o, lse, algo):
     nbytes = _attn_paged_bytes(idx, code, batch, T, heads, hkv, hd, shared)
     # the call's own scratch, from torch's stream-ordered allocator: calls on other streams
     # and captured graphs never share it
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = lens.new_empty(nbytes // 4)
     rc = _lib().pe_attn_paged(
         code, batch, T, heads, hkv, hd, q.data_ptr(), _row_stride(q), k_cache.data_ptr(),
         v_cache.data_ptr(), pages, page, table.data_ptr(), table_ld, table.shape[1],
