@@ -379,6 +379,18 @@ bool prefix_per_request(bool tc, int64_t B, int64_t rows, int64_t keys) {
   return B * keys <= (tc ? 700000 : 160000);
 }
 
+// Whether no entity is cut: requests that cannot be long (the block table's width says so)
+// are worth neither partial results nor the join's launch.  Device time of (uncut, cut) in us,
+// bf16, 28/4 heads of 128, requests of up to as many keys:
+//   1 row:   1 request   256 keys 9, 13    512 12, 13    1024 14, 14
+//            16          256 keys 11, 14   512 12, 16    1024 15, 17    2048 21, 19
+//            256         256 keys 46, 51   512 61, 66    1024 81, 82    2048 137, 136
+//   5 rows:  1 request   256 keys 13, 16   512 16, 16    1024 21, 18
+//            64          256 keys 23, 30   512 28, 35    1024 39, 43    2048 59, 57
+bool uncut(const Phase& p, int64_t keys, int64_t heads) {
+  return p.kind == kFew && (keys <= 640 || (keys <= 1024 && heads >= 64));
+}
+
 int64_t al256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // bytes of one phase's partial results
@@ -399,7 +411,7 @@ int run_phase(int dtype, const Phase& p, const Args& a, bool dependent, cudaStre
   const int rc = p.kind == kFew    ? launch_few(a, p.Mt, p.blocks, dependent, st)
                  : p.kind == kMany ? launch_many(a, p.blocks, dependent, st)
                                    : launch_simt(dtype, a, p.blocks, dependent, st);
-  if (rc) return rc;
+  if (rc || a.whole) return rc;
   return launch_join(dtype, a, p.blocks, p.Mt, st);
 }
 
@@ -501,6 +513,7 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     a.pre_lse = pre_lse;
   }
   const Phase p = tc ? tc_phase(ceil_div(T * a.G, B)) : simt_phase(dtype, hd);
+  a.whole = uncut(p, a.kmax - a.kbeg, B * Hkv);
   carve(a, p, ws);
   // The requests' own keys start while the prefix ends, unless it takes long (here: some 10
   // ms): nothing is gained then, and a block's bounded waits would run while it waits.

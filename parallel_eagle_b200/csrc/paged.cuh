@@ -11,8 +11,9 @@
 // A piece that is a whole entity writes its rows' result.  Otherwise an entity's pieces
 // leave partial results (accumulator, running maximum, sum) in per-block slots -- a block
 // has at most two incomplete entities, its first and its last -- and the block that holds
-// the entity's first piece records how many there are; the combine kernel joins them in
-// piece order, so results do not depend on timing.
+// the entity's first piece records how many there are; the join kernel adds them in
+// piece order, so results do not depend on timing.  (Where requests are short, no entity is
+// cut: a block takes those that start in its piece.)
 #pragma once
 #include <atomic>
 
@@ -36,6 +37,7 @@ struct Args {
   int64_t kbeg;           // first key (the shared prefix, when another launch does it)
   int all_rows;           // 1: one request of cu[B] rows that all see keys [kbeg, kmax)
   int align;              // 1: pieces that cut every entity at the same places (all_rows)
+  int whole;              // 1: a block takes the entities that start in its piece, uncut
   float scale_log2;       // log2(e) / sqrt(hd)
   void* o;                // result rows (the operand type), row stride o_ld
   int64_t o_ld;
@@ -231,6 +233,12 @@ struct Sched {
 
   // next segment of the piece; false when there is none.  Same result in every thread.
   __device__ __forceinline__ bool next() {
+    while (find()) {
+      if (!a.whole || first) return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool find() {
     if (pos >= end) return false;
     int64_t rc = req_cost(rq);
     while (pos >= base + rc) {  // (requests without rows cost nothing)
@@ -251,7 +259,7 @@ struct Sched {
     }
     rt = lo;
     const int64_t c = cost(rq, rt), u0 = off - cost_before(rq, rt);
-    const int64_t u1 = min(c, u0 + (end - pos));
+    const int64_t u1 = a.whole ? c : min(c, u0 + (end - pos));
     // the entity's key tiles, in proportion to its units
     const int rows_end = (int)min((int64_t)rq.n * a.G, (int64_t)(rt + 1) * Mt);
     const int last_tok = (rows_end - 1) / a.G;

@@ -627,3 +627,17 @@ def test_prefix_beyond_the_cache():
     lens, news = [shared + 9 + 30 * i for i in range(20)], [5] * 20
     case = make(lens, news, 40, 8, 128, 128, BF16, shared=shared)
     check(*case, 40, *attend(case, shared=shared))
+
+
+@pytest.mark.parametrize("width", [600, 640, 656, 1024, 1040])
+def test_widths_where_entities_are_cut_or_not(width):
+    """The same requests under block tables of other widths (which say how long requests can
+    be, and so whether blocks share one): the results agree with the definition in each."""
+    lens = [min(width, 37 + 61 * i) for i in range(20)]
+    for news in ([1] * 20, [5] * 20):
+        q, kc, vc, table, ln, cu = make(lens, news, 28, 4, 128, 16, BF16, seed=width)
+        wide = torch.full((20, -(-width // 16)), 2**31 - 1, dtype=torch.int32, device=DEV)
+        n = min(wide.shape[1], table.shape[1])
+        wide[:, :n] = table[:, :n]
+        case = (q, kc, vc, wide, ln, cu)
+        check(*case, 28, *attend(case))
