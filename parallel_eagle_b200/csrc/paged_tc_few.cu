@@ -31,7 +31,7 @@
 // Measured (28/4 heads of 128, device time with the join): 64 requests x 1 row, 1.1M keys in
 // all, 331 us, 6.7 TB/s -- the rate of a plain copy; 8 drafts of 5..9 rows, 36K keys in all,
 // 30.6 us, of which 10 us are the tiles, 6 us the way to the first scores (lengths, then
-// block table, then keys), 3 us the results and 4 us the join; one row over 600 keys 12 us.
+// block table, then keys), 3 us the results and 4 us the join; one row over 600 keys 11.6 us.
 // Code that runs once per segment is kept short (rolled loops): its time is mostly the
 // instructions' way from L2 (an unrolled epilogue made the drafts 39 us).
 #include "paged.cuh"
