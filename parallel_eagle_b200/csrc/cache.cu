@@ -282,9 +282,10 @@ extern "C" int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_
   PE_CHECK_ARG(ring != ring_out && lens != granted && new_lens != granted,
                "cache_plan: ring_out and granted must not alias the inputs");
   const size_t smem = (5 * (size_t)B + 3) * sizeof(int);
-  if (smem > 48 * 1024)
-    PE_CUDA_TRY(cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)smem));
+  if (smem > 48 * 1024) {
+    const int rc = allow_smem<plan_kernel>((5 * kPlanBatch + 3) * (int)sizeof(int));
+    if (rc) return rc;
+  }
   // a block per 1024 rows (and per 256 requests, whose pages it fills), up to three per SM:
   // a row's chain of dependent reads takes the time, so the more in flight the better
   // (512 prompts, 811K rows: 14 us with three, 23 us with one and a row a thread)

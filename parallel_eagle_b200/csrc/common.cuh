@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -83,6 +84,22 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // number of SMs of the current device (cached per device)
 int sm_count();
+
+// Let kernel K use `bytes` of dynamic shared memory, once per device: the runtime's call costs
+// as much as a quarter of a launch.  The limit is the kernel's, not the launch's, so `bytes` is
+// what its largest launch needs: a limit that followed each call's own size would be lowered by
+// one host thread between another one's setting and its launch.
+template <auto K>
+inline int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int dev = 0;
+  PE_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return PE_OK;
+  PE_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return PE_OK;
+}
 
 // Library-owned non-blocking stream of the current device (slot 0..3), created on
 // first use; kernels independent of the caller's stream run there and are joined

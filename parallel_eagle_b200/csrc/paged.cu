@@ -330,7 +330,8 @@ int launch_simt(int dtype, const Args& a, int blocks, bool dependent, cudaStream
                   (reinterpret_cast<uintptr_t>(a.vc) & 15u) == 0;
   return PE_DISPATCH(dtype, T, [&]() -> int {
     auto kern = paged_simt_kernel<T>;
-    PE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int rc = allow_smem<paged_simt_kernel<T>>((int)simt_smem(256, sizeof(T)));
+    if (rc) return rc;
     return launch_kernel(kern, dim3((unsigned)blocks), kThreads, smem, st, dependent, a, hdp, vec);
   });
 }

@@ -15,8 +15,6 @@
 // piece order, so results do not depend on timing.  (Where requests are short, no entity is
 // cut: a block takes those that start in its piece.)
 #pragma once
-#include <atomic>
-
 #include "common.cuh"
 
 namespace pe {
@@ -329,20 +327,6 @@ __device__ __forceinline__ void start_next_kernel() {
 }
 __device__ __forceinline__ void wait_kernel_before() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-// Let kernel K use `bytes` of dynamic shared memory (always the same number), once per device:
-// the runtime's call costs as much as a quarter of a launch.
-template <auto K>
-inline int allow_smem(int bytes) {
-  static std::atomic<uint64_t> done{0};  // a bit per device
-  int dev = 0;
-  PE_CUDA_TRY(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (bit && (done.load(std::memory_order_relaxed) & bit)) return PE_OK;
-  PE_CUDA_TRY(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return PE_OK;
 }
 
 // launch, optionally as a dependent of the kernel before it in the stream

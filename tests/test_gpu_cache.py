@@ -14,6 +14,7 @@
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 import torch
@@ -641,3 +642,68 @@ def test_widths_where_entities_are_cut_or_not(width):
         wide[:, :n] = table[:, :n]
         case = (q, kc, vc, wide, ln, cu)
         check(*case, 28, *attend(case))
+
+
+def _from_threads(calls, times):
+    """Each C call in a loop of its own host thread and stream, all at once (ctypes lets go of
+    the interpreter's lock, so the library's host code runs in parallel)."""
+    failed = []
+    start = threading.Barrier(len(calls))
+
+    def loop(fn, args):
+        with torch.cuda.device(DEV):
+            stream = torch.cuda.Stream()
+            args = (*args, stream.cuda_stream)
+            start.wait()
+            for _ in range(times):
+                if fn(*args):
+                    failed.append(L.load().pe_last_error().decode())
+                    break
+            stream.synchronize()
+
+    threads = [threading.Thread(target=loop, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
+def test_plans_of_two_sizes_from_several_threads():
+    """Batches whose scans need different amounts of shared memory, planned at once."""
+    lib, calls, keep = L.load(), [], []
+    for batch in (8000, 3000, 8000, 3000):
+        zero, table, granted = (torch.zeros(batch, dtype=torch.int32, device=DEV)
+                                for _ in range(3))
+        free, cu = _i32([0]), torch.empty(batch + 1, dtype=torch.int32, device=DEV)
+        ring, out = (torch.tensor([0, 1, 0], device=DEV) for _ in range(2))
+        row = torch.empty(1, dtype=torch.int64, device=DEV)
+        ts = (zero, table, granted, free, cu, ring, out, row)
+        keep.append(ts)
+        z, t, g, f, c, r, o, w = (x.data_ptr() for x in ts)
+        calls.append((lib.pe_cache_plan, (batch, 1, 1, 16, 0, 0, z, z, t, 1, f, r, o, g, c, w, w)))
+    torch.cuda.synchronize()
+    _from_threads(calls, 5000)
+    for zero, _, granted, *_ in keep:
+        assert torch.equal(zero, granted)
+
+
+def test_head_sizes_from_several_threads():
+    """fp32 attention over two head sizes at once: their tiles' shared memory differs."""
+    lib, calls, keep = L.load(), [], []
+    for hd in (256, 64, 256, 64):
+        case = make([90, 40], [2, 1], 2, 2, hd, 16, F32, seed=hd)
+        q, kc, vc, table, lens, cu = case
+        o, lse = torch.empty_like(q), torch.empty(2, 3, device=DEV)
+        nbytes = lib.pe_attn_paged_workspace(L.F32, 2, 3, 2, 2, hd, 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+        ln, c = _i32(lens), _i32(cu)
+        keep.append((case, o, lse, ws, ln, c))
+        calls.append((lib.pe_attn_paged, (
+            L.F32, 2, 3, 2, 2, hd, q.data_ptr(), 2 * hd, kc.data_ptr(), vc.data_ptr(), kc.shape[0],
+            16, table.data_ptr(), table.shape[1], table.shape[1], ln.data_ptr(), c.data_ptr(), 0,
+            o.data_ptr(), 2 * hd, lse.data_ptr(), ws.data_ptr(), nbytes, 0, None)))
+    torch.cuda.synchronize()
+    _from_threads(calls, 5000)
+    for case, o, lse, *_ in keep:
+        check(*case, 2, o, lse)
