@@ -50,6 +50,10 @@ const char* pe_last_error(void);
 int pe_version(void);
 /* number of kernels this library launched since load (for launch accounting) */
 int64_t pe_launch_count(void);
+/* Set the calling thread's stream-capture mode (0 global, 1 thread-local, 2 relaxed) and return
+ * the one before in *mode: what a host needs to allocate memory that is no part of the graph
+ * being captured. */
+int pe_exchange_capture_mode(int* mode);
 
 /* ---------------------------------------------------------------------------
  * RMSNorm  y = (x * rsqrt(mean(x^2) + eps)) * w, computed in fp32.

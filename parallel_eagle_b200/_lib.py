@@ -17,6 +17,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libpe_b200.so"
 F32, BF16, F16 = 0, 1, 2
 ALGO_AUTO, ALGO_SIMT, ALGO_TCGEN05 = 0, 1, 2
 PAGED_PREFIX_ONCE = 0x100
+CAPTURE_RELAXED = 2
 LAYOUT_PARTITION, LAYOUT_INDEXED, LAYOUT_BIAS = 0, 1, 2
 
 _vp, _i64, _f32, _int, _sz = C.c_void_p, C.c_int64, C.c_float, C.c_int, C.c_size_t
@@ -26,6 +27,7 @@ SIGNATURES: dict[str, tuple] = {
     "pe_last_error": (C.c_char_p, []),
     "pe_version": (_int, []),
     "pe_launch_count": (_i64, []),
+    "pe_exchange_capture_mode": (_int, [_vp]),
     "pe_rmsnorm_fwd": (_int, [_int, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _f32, _vp]),
     "pe_rmsnorm_bwd": (
         _int,

@@ -71,3 +71,10 @@ cudaEvent_t pool_event(int i) {
 extern "C" const char* pe_last_error(void) { return pe::g_last_error.c_str(); }
 extern "C" int pe_version(void) { return 1; }
 extern "C" int64_t pe_launch_count(void) { return pe::launch_counter(); }
+extern "C" int pe_exchange_capture_mode(int* mode) {
+  PE_CHECK_ARG(mode && *mode >= 0 && *mode <= 2, "exchange_capture_mode: mode must be 0, 1 or 2");
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(*mode);
+  PE_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&m));
+  *mode = static_cast<int>(m);
+  return PE_OK;
+}

@@ -7,6 +7,7 @@ allocated here (torch owns all memory); the library itself never allocates.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 
@@ -18,14 +19,31 @@ from . import _lib as L
 _status: dict[int, torch.Tensor] = {}
 
 
+@contextlib.contextmanager
+def _relaxed_capture():
+    """This thread may allocate and wait meanwhile, although a stream is being captured."""
+    mode = ctypes.c_int(L.CAPTURE_RELAXED)
+    L.check(_lib().pe_exchange_capture_mode(ctypes.byref(mode)), "pe_exchange_capture_mode")
+    try:
+        yield
+    finally:
+        L.check(_lib().pe_exchange_capture_mode(ctypes.byref(mode)), "pe_exchange_capture_mode")
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 word the tensor-core kernels write a code into when a
     bounded wait times out (0 = healthy)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status.get(idx)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _status[idx] = t
+        # on a stream of its own: when the caller's is being captured, neither the memory nor
+        # its clearing may become part of the graph
+        with _relaxed_capture():
+            side = torch.cuda.Stream(idx)
+            with torch.cuda.stream(side):
+                t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+            side.synchronize()
+        t = _status.setdefault(idx, t)
     return t
 
 

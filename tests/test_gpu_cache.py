@@ -707,3 +707,24 @@ def test_head_sizes_from_several_threads():
     _from_threads(calls, 5000)
     for case, o, lse, *_ in keep:
         check(*case, 2, o, lse)
+
+
+def test_first_call_under_capture_leaves_the_status_word_alone(monkeypatch):
+    """A device's status word that a capture creates is no part of the graph: its replays do
+    not clear what a kernel recorded, and it is healthy before the first of them."""
+    case = make([40, 9], [2, 1], 4, 2, 64, 16, BF16)
+    q, kc, vc, table, lens, cu = case
+    ln, c = _i32(lens), _i32(cu)
+    ops.attn_paged(q, kc, vc, table, ln, c)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(ops, "_status", {})
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o, lse = ops.attn_paged(q, kc, vc, table, ln, c)
+    ops.check_status(DEV)
+    ops.status_word(DEV).fill_(7)
+    g.replay()
+    with pytest.raises(L.PeError, match="fault code 7"):
+        ops.check_status(DEV)
+    ops.check_status(DEV)
+    check(*case, 4, o, lse)
