@@ -77,9 +77,14 @@ class DraftCache:
         rows = sum(max(0, w - h) for h, w in zip(self.lengths, lengths))
         want = torch.tensor(lengths, dtype=torch.int32).to(self.lens.device)
         with torch.cuda.device(self.lens.device):
+            lens, ring = self.lens, self._ring
             self.lens, cu, slots, pos, self._ring = ops.cache_plan(
-                self.lens, want, self.table, self._free, self._ring, self.page, rows,
-                shared=self.shared)
+                lens, want, self.table, self._free, ring, self.page, rows, shared=self.shared)
+            # they may be another stream's memory (the one the cache was used on before), which
+            # must not give them to others while this stream still reads them
+            stream = torch.cuda.current_stream()
+            lens.record_stream(stream)
+            ring.record_stream(stream)
         self.lengths = list(lengths)
         self.free_pages += back - need
         return cu, slots, pos

@@ -164,3 +164,27 @@ def test_refusals_leave_the_cache_as_it_was():
     assert cache.lengths == have
     _check_pages(cache)
     _round(model, cache, seqs, have, [1, 2], 4, tol)
+
+
+def test_cache_moves_to_another_stream(monkeypatch):
+    """Lengths and ring that a resize replaces are not given to the stream they came from while
+    the stream that plans still reads them."""
+    model, _, _ = _model(0, 20, 1)
+    cache = DraftCache(model, 2, pages=8, page=16)
+    plan = ops.cache_plan
+
+    def late_plan(*args, **kw):
+        torch.cuda._sleep(100_000_000)
+        return plan(*args, **kw)
+
+    monkeypatch.setattr(ops, "cache_plan", late_plan)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        cu, slots, pos = cache.resize([20, 5])
+    junk = [torch.full((6,), 77, dtype=torch.int32, device=DEV) for _ in range(200)]
+    torch.cuda.synchronize()
+    assert cache.lens.tolist() == [20, 5] and cu.tolist() == [0, 20, 25]
+    assert pos.tolist() == [*range(20), *range(5)] and slots.min() >= 0
+    _check_pages(cache)
+    assert all((j == 77).all() for j in junk)
