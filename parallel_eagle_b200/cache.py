@@ -97,13 +97,15 @@ class DraftCache:
         self.resize([length if b == request else n for b, n in enumerate(self.lengths)])
 
     def finish(self, request: int) -> None:
-        """Give the pages of ``request`` back; the number can be used for a new request."""
+        """Give the pages of ``request`` back, all but a shared prefix's; the number can be used
+        for a new request."""
         self.truncate(request, self.shared)
 
     def set_prefix(self, drafter, ids: torch.Tensor, features: torch.Tensor) -> int:
         """Compute the whole pages of a prompt once, for all requests: every request then
         starts behind them.  Returns how many of its tokens they hold; the rest of the
-        prompt is each request's own.  The cache has to be empty."""
+        prompt is each request's own.  The cache has to be empty (:meth:`drop_prefix` gives
+        an earlier prefix back)."""
         if any(self.lengths) or self.shared:
             raise ValueError("the shared prefix is set on an empty cache")
         n = ids.shape[0] // self.page * self.page
@@ -115,3 +117,16 @@ class DraftCache:
             self.lengths = [n] * self.requests
             self.shared = n
         return n
+
+    def drop_prefix(self) -> None:
+        """Give the shared prefix's pages back, for another one or none; every request has to
+        be finished."""
+        if any(n != self.shared for n in self.lengths):
+            raise ValueError(f"the shared prefix of {self.shared} keys is dropped once every "
+                             f"request is finished, not at lengths {self.lengths}")
+        if self.shared:
+            # its pages become request 0's own, which gives them back once
+            self.lens[1:].zero_()
+            self.lengths[1:] = [0] * (self.requests - 1)
+            self.shared = 0
+            self.resize([0] * self.requests)

@@ -188,3 +188,31 @@ def test_cache_moves_to_another_stream(monkeypatch):
     assert pos.tolist() == [*range(20), *range(5)] and slots.min() >= 0
     _check_pages(cache)
     assert all((j == 77).all() for j in junk)
+
+
+def test_prefixes_one_after_another():
+    """A prefix is given back when its requests are finished, and the next one takes its pages."""
+    model, seqs, tol = _model(1, 140, 3)
+    cache = DraftCache(model, 3, pages=14, page=16, max_len=112)
+    free = cache.free_pages
+    cache.drop_prefix()  # there is none
+    for prompt, own in ((75, 9), (33, 30), (90, 2)):
+        for b in range(3):
+            seqs[b] = tuple(torch.cat([seqs[-1][j][:prompt], seqs[b][j][prompt:]]) for j in (0, 1))
+        n = cache.set_prefix(model, seqs[0][0][:prompt], seqs[0][1][:prompt])
+        assert n == prompt // 16 * 16 and cache.free_pages == free - n // 16
+        have = [n] * 3
+        _round(model, cache, seqs, have, [prompt - n + own, 0, prompt - n + 1], 5, tol)
+        _check_pages(cache)
+        with pytest.raises(ValueError, match="finished"):
+            cache.drop_prefix()
+        for b in range(3):
+            cache.finish(b)
+        _check_pages(cache)
+        cache.drop_prefix()
+        assert cache.shared == 0 and cache.lengths == [0] * 3 and cache.free_pages == free
+        assert cache.lens.tolist() == [0] * 3
+        _check_pages(cache)
+    have = [0] * 3
+    _round(model, cache, seqs, have, [40, 7, 20], 4, tol)  # and without one
+    _check_pages(cache)
