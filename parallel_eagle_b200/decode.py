@@ -65,26 +65,31 @@ def propose_trees(drafter, cache, ids: torch.Tensor, feats: torch.Tensor, news: 
     """:func:`propose_tree` for every request of a :class:`cache.DraftCache` that has new
     confirmed tokens (``news[b]`` of them, in ``ids`` and ``feats`` one request after
     another): one drafter pass over the new tokens and prediction slots of all requests,
-    one selection launch."""
+    one selection launch.  Raises :class:`PeError` if a kernel gave up waiting; the cache's
+    new keys are then not to be used (``truncate`` takes them back)."""
     if k <= 0:
         raise ValueError(f"k must be positive, got {k}")
     logits = drafter.draft_logits_cached(cache, ids, feats, news, k)
     beam_width = max(1, min(top_k, max_nodes // k))
     vals, toks = ops.topk_logprobs(logits.flatten(0, 1), beam_width)
     shape = (logits.shape[0], k, beam_width)
-    return [_grow_tree(v, t, k, beam_width)
-            for v, t in zip(vals.view(shape).tolist(), toks.view(shape).tolist())]
+    vals, toks = vals.view(shape).tolist(), toks.view(shape).tolist()
+    ops.check_status(logits.device)
+    return [_grow_tree(v, t, k, beam_width) for v, t in zip(vals, toks)]
 
 
 def propose_chains(drafter, cache, ids: torch.Tensor, feats: torch.Tensor, news: list[int],
                    k: int) -> list[list[int]]:
     """:func:`propose_chain` for every request of a :class:`cache.DraftCache` that has new
-    confirmed tokens: one drafter pass and one selection launch for all of them."""
+    confirmed tokens: one drafter pass and one selection launch for all of them.  Raises as
+    :func:`propose_trees` does."""
     if k <= 0:
         raise ValueError(f"k must be positive, got {k}")
     logits = drafter.draft_logits_cached(cache, ids, feats, news, k)
     _, toks = ops.topk_logprobs(logits.flatten(0, 1), 1, raw=True)
-    return toks.view(-1, k).tolist()
+    toks = toks.view(-1, k).tolist()
+    ops.check_status(logits.device)
+    return toks
 
 
 def propose_chain_sequential(drafter, context_ids: torch.Tensor, context_feats: torch.Tensor,

@@ -216,3 +216,24 @@ def test_prefixes_one_after_another():
     have = [0] * 3
     _round(model, cache, seqs, have, [40, 7, 20], 4, tol)  # and without one
     _check_pages(cache)
+
+
+def test_proposals_report_a_kernel_that_gave_up():
+    """What a bounded wait records reaches the caller with the drafts of that call, once."""
+    model, seqs, _ = _model(1, 60, 2)
+    cache = DraftCache(model, 2, pages=20, page=16)
+    ids, feats = (torch.cat([s[j][:9] for s in seqs]) for j in (0, 1))
+    calls = [lambda: decode.propose_trees(model, cache, ids, feats, [9, 9], 4, 2, 8),
+             lambda: decode.propose_chains(model, cache, ids, feats, [9, 9], 4)]
+    for call in calls:
+        want = call()
+        cache.truncate(0, 0)
+        cache.truncate(1, 0)
+        ops.status_word(DEV).fill_(403)
+        with pytest.raises(L.PeError, match="fault code 403"):
+            call()
+        cache.truncate(0, 0)
+        cache.truncate(1, 0)
+        assert call() == want
+        cache.truncate(0, 0)
+        cache.truncate(1, 0)
