@@ -268,7 +268,7 @@ extern "C" int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_
   PE_CHECK_ARG(B >= 1 && B <= kPlanBatch, "cache_plan: %lld requests, expected 1 to %d",
                (long long)B, kPlanBatch);
   PE_CHECK_ARG(page >= 1 && page <= (1 << 20), "cache_plan: page size %lld", (long long)page);
-  PE_CHECK_ARG(width >= 1 && width * page < (1ll << 31) && table_ld >= width,
+  PE_CHECK_ARG(width >= 1 && width < (1ll << 31) && width * page < (1ll << 31) && table_ld >= width,
                "cache_plan: block table of %lld pages (row stride %lld)", (long long)width,
                (long long)table_ld);
   PE_CHECK_ARG(num_pages >= 1 && num_pages < (1ll << 30) && B * width < (1ll << 31),
@@ -305,10 +305,11 @@ extern "C" int pe_cache_append(int dtype, int64_t rows, int Hkv, int hd, const v
                                void* stream) {
   PE_CHECK_ARG(dtype == PE_F32 || dtype == PE_BF16, "cache_append: unsupported dtype code %d",
                dtype);
-  PE_CHECK_ARG(rows >= 0 && Hkv >= 1 && hd >= 1 && (int64_t)Hkv * hd < (1 << 24),
+  PE_CHECK_ARG(rows >= 0 && rows < (1ll << 38) && Hkv >= 1 && hd >= 1 &&
+                   (int64_t)Hkv * hd < (1 << 24),
                "cache_append: %lld rows of %d heads of %d", (long long)rows, Hkv, hd);
-  PE_CHECK_ARG(num_pages >= 0 && page >= 1 && page <= (1 << 20), "cache_append: %lld pages of %lld",
-               (long long)num_pages, (long long)page);
+  PE_CHECK_ARG(num_pages >= 0 && num_pages < (1ll << 31) && page >= 1 && page <= (1 << 20),
+               "cache_append: %lld pages of %lld", (long long)num_pages, (long long)page);
   if (rows == 0) return PE_OK;
   PE_CHECK_ARG(k && v && slots && k_cache && v_cache, "cache_append: null pointer");
   PE_CHECK_ARG(rows == 1 || (k_ld >= (int64_t)Hkv * hd && v_ld >= (int64_t)Hkv * hd),

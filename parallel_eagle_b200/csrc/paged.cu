@@ -450,11 +450,12 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
   PE_CHECK_ARG(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 256,
                "attn_paged: %d query heads over %d KV heads", Hq, Hkv);
   PE_CHECK_ARG(hd >= 1 && hd <= 256, "attn_paged: head_dim %d, expected 1 to 256", hd);
-  PE_CHECK_ARG(B >= 1 && B < (1 << 20) && T >= 0 && T * Hq < (1ll << 31),
+  PE_CHECK_ARG(B >= 1 && B < (1 << 20) && T >= 0 && T < (1ll << 31) && T * Hq < (1ll << 31),
                "attn_paged: %lld requests, %lld rows of %d heads", (long long)B, (long long)T, Hq);
   PE_CHECK_ARG(page >= 16 && page % 16 == 0 && page <= (1 << 20),
                "attn_paged: page size %lld is not a multiple of 16", (long long)page);
-  PE_CHECK_ARG(num_pages >= 1 && num_pages < (1ll << 31) && num_pages * Hkv * page < (1ll << 40),
+  PE_CHECK_ARG(num_pages >= 1 && num_pages < (1ll << 31) &&
+                   num_pages * page < ceil_div(1ll << 40, Hkv),
                "attn_paged: %lld pages", (long long)num_pages);
   PE_CHECK_ARG(width >= 1 && width <= (1 << 27) / page && table_ld >= width,
                "attn_paged: block table of %lld pages (row stride %lld)", (long long)width,

@@ -108,3 +108,22 @@ def test_draft_cache_needs_a_gpu():
     for max_len in (0, -5):
         with pytest.raises(ValueError, match="max_len"):
             DraftCache(d, 1, 4, max_len=max_len)
+
+
+def test_sizes_whose_products_wrap_are_refused():
+    """Sizes so large that a product of them passes 2^63 are refused like any other too large
+    ones, before anything is launched."""
+    lib = _lib.load()
+    big = 1 << 62
+    for kw in (dict(width=big, table_ld=big, page=16), dict(width=1 << 61, table_ld=1 << 61, B=8)):
+        assert _plan(lib, **kw) == 1, kw
+        assert b"cache_plan" in lib.pe_last_error()
+    for kw in (dict(pages=big), dict(pages=1 << 60, page=1 << 20), dict(rows=big),
+               dict(rows=1 << 57, Hkv=1)):
+        assert _append(lib, **kw) == 1, kw
+        assert b"cache_append" in lib.pe_last_error()
+    for kw in (dict(T=big), dict(T=1 << 61, Hq=8, q_ld=512, o_ld=512),
+               dict(pages=(1 << 31) - 1, Hq=1 << 14, Hkv=1 << 14, page=1 << 20, q_ld=1 << 20,
+                    o_ld=1 << 20)):
+        assert _attn(lib, **kw) == 1, kw
+        assert b"attn_paged" in lib.pe_last_error()
