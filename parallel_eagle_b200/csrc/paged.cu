@@ -48,8 +48,15 @@ inline size_t simt_smem(int hdp, int es) {
   return 4ull * kTK * simt_ld(hdp, es) * es + (size_t)kSimtRows * (hdp + 4 + kLdP) * sizeof(float);
 }
 
+// Blocks that an SM's registers hold: 128 a thread for fp32, 160 for bf16 (whose conversions
+// want more).  The grid is one wave of them, as all pieces are equal.  With a fourth bf16 block
+// an SM, which waits for a place, 64 tokens over up to 4K keys took 237 us, 132 with three
+// (12/3 heads of 80), and 804 against 450 (16/16 heads of 40).
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+constexpr int kSimtBlocks = sizeof(T) == 4 ? 4 : 3;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kSimtBlocks<T>)
 paged_simt_kernel(const __grid_constant__ Args a, int hdp, int vec) {
   constexpr int Mt = kSimtRows;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -345,9 +352,11 @@ struct Phase {
 };
 
 Phase simt_phase(int dtype, int hd) {
-  // as many blocks as the tiles' shared memory lets an SM hold, four at most
+  // as many blocks as the tiles' shared memory and the registers let an SM hold
   const size_t smem = simt_smem((hd + 3) / 4 * 4, dtype == PE_F32 ? 4 : 2);
-  return {kSimt, kSimtRows, sm_count() * (int)std::max<size_t>(1, std::min<size_t>(4, 220 * 1024 / smem))};
+  const size_t most = dtype == PE_F32 ? kSimtBlocks<float> : kSimtBlocks<__nv_bfloat16>;
+  return {kSimt, kSimtRows,
+          sm_count() * (int)std::max<size_t>(1, std::min<size_t>(most, 220 * 1024 / smem))};
 }
 
 // tensor-core kernel for `rows` packed rows (on average) per request and KV head

@@ -127,3 +127,14 @@ def test_sizes_whose_products_wrap_are_refused():
                     o_ld=1 << 20)):
         assert _attn(lib, **kw) == 1, kw
         assert b"attn_paged" in lib.pe_last_error()
+
+
+def test_cuda_core_grid_is_one_wave():
+    """The partial results of a call (two a block, 16 rows of head_dim + 2 floats) are those of
+    the blocks that the GPU holds at once: registers allow three an SM for bf16, four for fp32
+    (148 SMs)."""
+    lib = _lib.load()
+    for dtype, blocks, hd in ((BF16, 3, 80), (BF16, 3, 40), (F32, 4, 80)):
+        per_block = 2 * 16 * (hd + 2) * 4
+        most = 148 * blocks * (per_block + 64)
+        assert lib.pe_attn_paged_workspace(dtype, 4, 4, 4, 2, hd, 0) <= most + 3 * 256
