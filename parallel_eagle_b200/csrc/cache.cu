@@ -26,8 +26,9 @@ namespace {
 // from the ring when this call is the one that takes it, so no block reads what another
 // writes and one launch does it all.  A thread describes two rows (one bisection, 16-byte
 // stores).  Bound by latency: a scan, then per row a bisection and one dependent read of the
-// ring or the table.  Measured: 8 drafts 5.2 us, 512 requests with 811K new rows 14 us.
+// ring or the table.  Measured: 8 drafts 5.2 us, 512 requests with 788K new rows 11 us.
 constexpr int kPlanThreads = 512;
+constexpr int kPlanBlocks = 2;    // blocks an SM's registers hold (60 a thread)
 constexpr int kPlanBatch = 8192;  // requests whose scan fits the block's shared memory
 
 struct Scan3 {
@@ -49,7 +50,7 @@ __device__ __forceinline__ int find(const int* v, int n, int x) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
+__global__ void __launch_bounds__(kPlanThreads, kPlanBlocks)
 plan_kernel(int B, int64_t width, int N, int page, int64_t rows, int sp,
             const int32_t* __restrict__ lens, const int32_t* __restrict__ want,
             int32_t* table, int64_t table_ld, int32_t* ring_pages,
@@ -286,11 +287,13 @@ extern "C" int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_
     const int rc = allow_smem<plan_kernel>((5 * kPlanBatch + 3) * (int)sizeof(int));
     if (rc) return rc;
   }
-  // a block per 1024 rows (and per 256 requests, whose pages it fills), up to three per SM:
-  // a row's chain of dependent reads takes the time, so the more in flight the better
-  // (512 prompts, 811K rows: 14 us with three, 23 us with one and a row a thread)
+  // a block per 1024 rows (and per 256 requests, whose pages it fills), up to what the SMs hold
+  // at once: a row's chain of dependent reads takes the time, so the more in flight the better,
+  // but a block that waits for a place starts with a scan of its own (512 prompts, 788K rows:
+  // 13.6 us with one an SM, 11.1 with two, 14.0 with three; 96K rows the same with each).
+  // Where the scan is long, one an SM: 4000 requests with 302K rows 21.3 us, 25.7 with two.
   const int64_t want = std::max(ceil_div(rows, 2 * kPlanThreads), ceil_div(B, 256));
-  const int64_t most = smem > 64 * 1024 ? 1 : 3;
+  const int64_t most = smem > 64 * 1024 ? 1 : kPlanBlocks;
   const int blocks = (int)std::min<int64_t>(std::max<int64_t>(want, 1), most * sm_count());
   plan_kernel<<<blocks, kPlanThreads, smem, as_stream(stream)>>>(
       (int)B, width, (int)num_pages, (int)page, rows, (int)(shared / page), lens, new_lens, table,

@@ -728,3 +728,9 @@ def test_first_call_under_capture_leaves_the_status_word_alone(monkeypatch):
         ops.check_status(DEV)
     ops.check_status(DEV)
     check(*case, 4, o, lse)
+
+
+@pytest.mark.parametrize("batch", [3200, 3300, 5600])
+def test_plan_scans_that_share_an_sm(batch):
+    """Many rows, with scans of which an SM runs two at once, or one."""
+    run_plan(*_plan_case(batch, 16, 16, 70000, seed=batch, head=5))
