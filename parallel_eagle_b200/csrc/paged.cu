@@ -391,14 +391,24 @@ bool prefix_per_request(bool tc, int64_t B, int64_t rows, int64_t keys) {
 
 // Whether no entity is cut: requests that cannot be long (the block table's width says so)
 // are worth neither partial results nor the join's launch.  Device time of (uncut, cut) in us,
-// bf16, 28/4 heads of 128, requests of up to as many keys:
-//   1 row:   1 request   256 keys 9, 13    512 12, 13    1024 14, 14
-//            16          256 keys 11, 14   512 12, 16    1024 15, 17    2048 21, 19
-//            256         256 keys 46, 51   512 61, 66    1024 81, 82    2048 137, 136
-//   5 rows:  1 request   256 keys 13, 16   512 16, 16    1024 21, 18
-//            64          256 keys 23, 30   512 28, 35    1024 39, 43    2048 59, 57
+// bf16, requests of up to as many keys, by heads of all requests (B * Hkv):
+//   1 row,  28/4 heads of 128:  4  512 keys 11, 13   640 12, 13    768 13, 14   1024 14, 15
+//                              64  512 keys 12, 16   640 13, 17    768 14, 17   1024 16, 18
+//                             256  512 keys 22, 26   640 24, 28    768 26, 31   1024 32, 35
+//   5 rows, 28/4 heads of 128:  4  512 keys 16, 16   640 17, 16    768 18, 16   1024 20, 18
+//   (35 packed: 64-row tiles)  16  512 keys 16, 18   640 17, 18    768 18, 19   1024 21, 20
+//                              64  512 keys 17, 20   640 18, 21    768 19, 21   1024 22, 23
+//   5 rows, 14/2 heads of 64:   2  512 keys 15, 15   640 16, 15    768 17, 15   1024 19, 17
+//   (the same)                  8  512 keys 15, 16   640 17, 17    768 18, 17   1024 20, 18
+//                              32  512 keys 16, 17   640 17, 19    768 18, 19   1024 20, 19
+//   5 rows, 40/8 heads of 128:  8  512 keys 13, 15   640 14, 16    768 15, 16   1024 17, 17
+//   (25 packed: 32-row tiles) 128  512 keys 15, 22   640 17, 23    768 18, 24   1024 21, 26
+// A 64-row tile takes longer per key, so few heads are cut earlier.  (2048 keys: 21, 19 for 64
+// heads of one row; 59, 57 for 256 heads of five.)
 bool uncut(const Phase& p, int64_t keys, int64_t heads) {
-  return p.kind == kFew && (keys <= 640 || (keys <= 1024 && heads >= 64));
+  if (p.kind != kFew) return false;
+  if (heads >= 64) return keys <= 1024;
+  return keys <= (p.Mt == 64 && heads < 16 ? 512 : 640);
 }
 
 int64_t al256(int64_t x) { return (x + 255) / 256 * 256; }

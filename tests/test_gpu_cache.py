@@ -734,3 +734,16 @@ def test_first_call_under_capture_leaves_the_status_word_alone(monkeypatch):
 def test_plan_scans_that_share_an_sm(batch):
     """Many rows, with scans of which an SM runs two at once, or one."""
     run_plan(*_plan_case(batch, 16, 16, 70000, seed=batch, head=5))
+
+
+@pytest.mark.parametrize("batch", [1, 3, 4])
+@pytest.mark.parametrize("width", [512, 528, 640, 656, 1024])
+def test_widths_where_few_requests_are_cut_or_not(batch, width):
+    """The same with few requests, whose tables' limit depends on the rows a tile holds."""
+    lens = [min(width, 500 + 13 * i) for i in range(batch)]
+    for n in (1, 4, 5, 9):  # 7 to 63 packed rows
+        q, kc, vc, table, ln, cu = make(lens, [n] * batch, 28, 4, 128, 16, BF16, seed=width + n)
+        wide = torch.full((batch, width // 16), 2**31 - 1, dtype=torch.int32, device=DEV)
+        wide[:, :min(wide.shape[1], table.shape[1])] = table[:, :wide.shape[1]]
+        case = (q, kc, vc, wide, ln, cu)
+        check(*case, 28, *attend(case))
