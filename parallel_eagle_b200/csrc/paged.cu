@@ -519,9 +519,15 @@ extern "C" int pe_attn_paged(int dtype, int64_t B, int64_t T, int Hq, int Hkv, i
     const Phase p = tc ? tc_phase(T * a.G) : simt_phase(dtype, hd);
     Args pa = a;
     pa.all_rows = 1;
-    // A prefix that L2 (126 MB) cannot keep: 64 samples over 64K keys, 268 MB, ran 562 us a
-    // call so and 606 us with equal pieces (sustained, under the power cap).
-    pa.align = 2 * shared * Hkv * hd * (dtype == PE_F32 ? 4 : 2) > (64ll << 20);
+    // Alike for a prefix that L2 (126 MB, in two halves) does not keep for all row tiles.  A
+    // call among others, sustained under the power cap, in us (equal pieces, aligned), samples
+    // of 5 rows:   64, 40/8 heads of 128:   64 MB 192, 199   128 MB 315, 320   256 MB 592, 577
+    //                                      512 MB 1129, 1079
+    //              64, 28/4 heads of 128:   64 MB 213, 212   128 MB 428, 365   256 MB 790, 686
+    //              32, the same:            64 MB 130, 126   128 MB 228, 213   256 MB 419, 384
+    // What it saves is the power that HBM takes: a few calls alone gain 5 % at most (28/4 heads)
+    // and lose 1 to 9 % (40/8).  (The CUDA-core kernel is bound by other things.)
+    pa.align = p.kind != kSimt && 4 * shared * Hkv * hd > (64ll << 20);
     pa.kmax = shared;
     pa.o32 = pre_o;
     pa.lse = pre_lse;

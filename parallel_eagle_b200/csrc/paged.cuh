@@ -34,7 +34,8 @@ struct Args {
   int B, T, Hq, Hkv, hd, G;  // G = Hq / Hkv
   int64_t kbeg;           // first key (the shared prefix, when another launch does it)
   int all_rows;           // 1: one request of cu[B] rows that all see keys [kbeg, kmax)
-  int align;              // 1: pieces that cut every entity at the same places (all_rows)
+  int align;              // 1: pieces that cut every entity at the same places (all_rows, and
+                          // the piece found by init_warp: the tensor-core kernels)
   int whole;              // 1: a block takes the entities that start in its piece, uncut
   float scale_log2;       // log2(e) / sqrt(hd)
   void* o;                // result rows (the operand type), row stride o_ld
