@@ -359,7 +359,17 @@ Phase simt_phase(int dtype, int hd) {
           sm_count() * (int)std::max<size_t>(1, std::min<size_t>(most, 220 * 1024 / smem))};
 }
 
-// tensor-core kernel for `rows` packed rows (on average) per request and KV head
+// Tensor-core kernel for `rows` packed rows (on average) per request and KV head: up to one tile
+// of the few-row kernel's largest kind; two of them read every key twice.  Device time of (few,
+// many) in us, bf16, requests of the same length:
+//   28/4 heads of 128,  8 x 8K:   42 rows 41, 48     63: 43, 49     77: 54, 48    126: 56, 51
+//                      64 x 4K:          100, 122       102, 122       174, 121       181, 129
+//                      64 x 600:          35, 51         37, 52         57, 51         58, 55
+//   40/8 heads of 128,  8 x 8K:   45 rows 59, 71     60: 60, 72     80: 86, 71    125: 89, 74
+//   6/6 heads of 64,   64 x 4K:   48 rows 124, 170   64: 127, 160   80: 223, 164
+// A single request, whose keys fill no SM for long, would be quicker with the few-row kernel up
+// to some hundred rows (1 x 1K, 126 rows: 20, 24), and a mean over requests of very different
+// rows fits none of them (requests without rows count in it, too); both are left so.
 Phase tc_phase(int64_t rows) {
   if (rows > 64) return {kMany, 256, sm_count()};
   return {kFew, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, sm_count()};
