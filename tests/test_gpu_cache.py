@@ -747,3 +747,104 @@ def test_widths_where_few_requests_are_cut_or_not(batch, width):
         wide[:, :min(wide.shape[1], table.shape[1])] = table[:, :wide.shape[1]]
         case = (q, kc, vc, wide, ln, cu)
         check(*case, 28, *attend(case))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("news", [1, 2, 5, 9])
+def test_shared_prefix_with_own_keys_in_pieces(news, hd):
+    """Own keys that blocks cut behind a prefix read once: the join of a request's pieces adds
+    the prefix's rows (7, 14, 35 and 63 packed rows: every kind of the few-row kernel)."""
+    shared, own = 1024, [700, 1100, 3000, 9, 2048]
+    case = make([shared + t for t in own], [news] * len(own), 28, 4, hd, 64, BF16,
+                seed=news + hd, shared=shared)
+    check(*case, 28, *attend(case, shared=shared))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_shared_prefix_with_prompts_behind_it(dtype, hd):
+    """The same with 40 to 300 new rows a request: whole tiles and pieces of the many-row
+    kernel (and of the CUDA-core one) behind the prefix."""
+    shared = 512
+    own, news = [300, 45, 1500, 400], [300, 40, 130, 77]
+    case = make([shared + t for t in own], news, 14, 2, hd, 16, dtype, seed=hd, shared=shared)
+    check(*case, 14, *attend(case, shared=shared))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_shared_prefix_repeats_and_is_right(dtype):
+    """Pieces of the prefix and of the own keys, joined in the same order every time."""
+    shared = 128
+    case = make([shared + 2500, shared + 31, shared + 800], [5, 3, 7], 28, 4, 128, 64, dtype,
+                shared=shared)
+    o, lse = attend(case, shared=shared)
+    check(*case, 28, o, lse)
+    for _ in range(3):
+        o2, l2 = attend(case, shared=shared)
+        assert torch.equal(o, o2) and torch.equal(lse, l2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("news", [1, 5, 33, 70])
+def test_many_requests_in_pieces(dtype, news):
+    """More than 128 requests (the whole block looks through them) under a table whose width
+    has them cut: most of them short, some over several blocks.  news 33 and 70: 66 and 140
+    packed rows, the many-row kernel."""
+    lens = [news + (17 * i) % 60 for i in range(150)]
+    for i in (0, 70, 149):
+        lens[i] = 4000 + 333 * i
+    q, kc, vc, table, ln, cu = make(lens, [news] * 150, 4, 2, 64, 64, dtype, seed=news)
+    assert table.shape[1] * 64 > 1024
+    case = (q, kc, vc, table, ln, cu)
+    check(*case, 4, *attend(case))
+
+
+@pytest.mark.parametrize("shared", [0, 64])
+def test_replay_beside_eager_calls(shared):
+    """A captured call replayed while eager calls run on another stream, with scratch of their
+    own: both are what they are alone."""
+    cases = [make([shared + 3000 + 500 * i, shared + 40], [5, 3], 28, 4, 128, 64, BF16,
+                  seed=20 + i, shared=shared) for i in range(2)]
+    fixed = [(c[:4], _i32(c[4]), _i32(c[5])) for c in cases]
+
+    def call(i):
+        args, ln, cu = fixed[i]
+        if shared:
+            return ops.attn_paged_shared(*args, ln, cu, shared, algo=L.PAGED_PREFIX_ONCE)
+        return ops.attn_paged(*args, ln, cu)
+
+    want = [call(i) for i in range(2)]
+    for case, (o, lse) in zip(cases, want):
+        check(*case, 28, o, lse)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        replayed = [call(0) for _ in range(8)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        g.replay()
+        with torch.cuda.stream(s):
+            eager = [call(1) for _ in range(8)]
+        torch.cuda.synchronize()
+        for (o, lse), got in ((want[0], replayed), (want[1], eager)):
+            for o2, l2 in got:
+                assert torch.equal(o, o2) and torch.equal(lse, l2)
+        for o2, _ in replayed:
+            o2.fill_(7)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shared", [0, 64])
+def test_mixed_batches(dtype, shared):
+    """A prompt beside single tokens, drafts and idle requests, under a table much wider than
+    any of them needs; whichever kernel the mean number of rows picks."""
+    for batch, prompt in ((64, 500), (12, 900)):
+        lens = [30 + 7 * i for i in range(batch)]
+        news = [(0, 1, 5, 0)[i % 4] for i in range(batch)]
+        lens[5], news[5] = prompt + 60, prompt
+        q, kc, vc, table, ln, cu = make([shared + t for t in lens], news, 28, 4, 128, 64, dtype,
+                                        seed=batch, shared=shared)
+        wide = torch.full((batch, 200), 2**31 - 1, dtype=torch.int32, device=DEV)
+        wide[:, :table.shape[1]] = table
+        case = (q, kc, vc, wide, ln, cu)
+        check(*case, 28, *attend(case, shared=shared))
