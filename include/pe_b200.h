@@ -382,7 +382,7 @@ int pe_cache_plan(int64_t B, int64_t width, int64_t num_pages, int64_t page, int
 
 /* Copy row t of k and v ([rows, Hkv * hd], row strides k_ld, v_ld) into cache slot slots[t];
  * rows with a slot outside [0, num_pages * page) are skipped.  Two rows with the same slot
- * leave either one's values. */
+ * leave a mixture of their values. */
 int pe_cache_append(int dtype, int64_t rows, int Hkv, int hd, const void* k, int64_t k_ld,
                     const void* v, int64_t v_ld, const int64_t* slots, int64_t num_pages,
                     int64_t page, void* k_cache, void* v_cache, void* stream);

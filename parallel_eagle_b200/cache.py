@@ -23,7 +23,8 @@ class DraftCache:
     ``max_len`` bounds a request's length, its prediction slots included (default: what the
     pages hold).  The host knows every length and the number of free pages, so running out
     raises :class:`PeError` before anything is launched; which pages a request holds is
-    planned on the device."""
+    planned on the device.  A step plans twice (its rows, then without its prediction slots),
+    each time from lengths that the host sends, so it cannot be captured; the operators can."""
 
     def __init__(self, drafter, requests: int, pages: int, page: int = 64,
                  max_len: int | None = None):

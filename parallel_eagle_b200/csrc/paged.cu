@@ -20,7 +20,7 @@ namespace {
 // products the tensor cores would round) and what the tensor-core kernels do not take.
 // Bound by shared-memory reads: a key's element is read once per 4 rows of a warp for the
 // scores and once for the output.  Measured: 16 requests of 1..5 rows, 17K keys in all, 4/2
-// heads of 64, fp32: 25.5 us with the join, of which half is a block's start, its one or two
+// heads of 64, fp32: 26.4 us with the join, of which half is a block's start, its one or two
 // results and the join.
 constexpr int kThreads = 128;
 constexpr int kSimtRows = 16;
@@ -386,12 +386,13 @@ bool tc_operands(const Args& a) {
 
 // Whether the requests read their common prefix each for itself.  Its pages then come from
 // L2 after the first time, and a prefix of its own costs two launches, an fp32 result and a
-// second start of the copies, 25 to 40 us.  Device time of (each for itself, once) in us,
+// second start of the copies.  Device time of (each for itself, once) in us,
 // by B * prefix keys * KV heads:
-//   bf16, 28/4 heads of 128, 1 row:   131K 20, 43   524K 36, 45   1.05M 56, 51   2.1M 102, 64
-//         5 rows:                     131K 27, 49   524K 51, 62   1.05M 84, 72   2.1M 155, 94
-//   bf16, 14/2 heads of 64, 5 rows:   131K 25, 45   524K 49, 55   1.05M 82, 65
-//   fp32, 4/2 heads of 64, 1 row:      66K 28, 39   131K 43, 45    262K 68, 55    524K 119, 63
+//   bf16, 28/4 heads of 128, 1 row:   131K 22, 30   524K 36, 41   1.05M 57, 48   2.1M 102, 59
+//         5 rows:                     131K 28, 43   524K 52, 59   1.05M 85, 66   2.1M 157, 89
+//   bf16, 14/2 heads of 64, 5 rows:   131K 27, 41   524K 50, 52   1.05M 83, 58
+//   fp32, 4/2 heads of 64, 1 row:      66K 27, 35   131K 37, 44    262K 54, 51    524K 93, 60
+//   bf16, 12/3 heads of 80, 1 row:     49K 34, 48   197K 57, 62    393K 96, 72
 // With more rows a request than the few-row kernel takes, the prefix's rows of all requests
 // fill its tiles better than each request's.
 bool prefix_per_request(bool tc, int64_t B, int64_t rows, int64_t keys) {

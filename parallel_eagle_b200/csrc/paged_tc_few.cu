@@ -28,10 +28,17 @@
 // TMEM: S^T 2 x N columns, O^T 2 x N (two segments: the next one starts while this one's
 // result is read).
 //
+// P is rounded to bf16, as the tensor core's operand has to be; its sum is not.  Each rounding
+// is off by at most 2^-8: results are 2.3e-3 (rms, relative) from 64 bits, 1.7e-3 of it the
+// result's own rounding.  (Another product with what the rounding leaves would take 16 KB of
+// shared memory and the value product's tensor work again.)
+//
 // Measured (28/4 heads of 128, device time with the join): 64 requests x 1 row, 1.1M keys in
-// all, 331 us, 6.7 TB/s -- the rate of a plain copy; 8 drafts of 5..9 rows, 36K keys in all,
-// 30.6 us, of which 10 us are the tiles, 6 us the way to the first scores (lengths, then
-// block table, then keys), 3 us the results and 4 us the join; one row over 600 keys 11.6 us.
+// all, 330 us, 6.7 TB/s -- the rate of a plain copy; 8 drafts of 5..9 rows, 36K keys in all,
+// 31 us: 6 us to a block's first scores (lengths, then block table, then keys), 10 us of
+// tiles, 2 us for a segment's results (the last block, which has two, ends 20.7 us after the
+// first one's start), 4 us the join, the rest the start and end of two launches; one row over
+// 600 keys 11.6 us, 12.5 under a wide table (cut, and joined).
 // Code that runs once per segment is kept short (rolled loops): its time is mostly the
 // instructions' way from L2 (an unrolled epilogue made the drafts 39 us).
 #include "paged.cuh"
@@ -482,7 +489,7 @@ paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             tmem_wait_st();
           }
         }
-        // probabilities, rounded to bf16 for the tensor core (their sum is not)
+        // probabilities, rounded to bf16 for the tensor core (their sum is not: see above)
         if (i > 0) bad |= !mbar_wait(&sm.p_empty, (i - 1) & 1, status, 414);
 #pragma unroll
         for (int u = 0; u < CW / 8; ++u) {

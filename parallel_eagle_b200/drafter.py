@@ -187,7 +187,12 @@ class ParallelDrafter(nn.Module):
 
         The rows see their request's cached keys and the rows before them: the partition
         layout with ``(a0, a1, K) = (p - 1, p, k)`` again, as the prediction slots follow the
-        last real one.  The prediction slots' keys are dropped afterwards."""
+        last real one.  The prediction slots' keys are dropped afterwards.
+
+        The pass reads the modules' weights and runs the kernels itself: forward hooks on the
+        layers, norms and projections, which :meth:`forward` fires, do not fire here.  It
+        returns without waiting for the GPU; :func:`ops.check_status` raises if a kernel gave
+        up waiting, and the request's new keys are then not to be used."""
         dev = self.device
         if len(news) != cache.requests or min(news) < 0 or sum(news) != ids.shape[0] \
                 or feats.shape[0] != ids.shape[0]:
@@ -248,7 +253,8 @@ class ParallelDrafter(nn.Module):
                             news: list[int], k: int) -> torch.Tensor:
         """:meth:`draft_logits` for a batch of requests whose context, all but the ``news[b]``
         last confirmed tokens, is in ``cache``: logits ``(requests with new tokens, k, V)``
-        for the ``k`` tokens that follow each.  ``cache`` then holds those tokens too."""
+        for the ``k`` tokens that follow each.  ``cache`` then holds those tokens too.  (Hooks
+        and errors: :meth:`forward_cached`.)"""
         hidden, first = self.forward_cached(cache, ids, feats, news, k)
         rows = [first[b] + n - 1 + d for b, n in enumerate(news) if n for d in range(k)]
         pick = torch.tensor(rows).to(hidden.device)

@@ -592,7 +592,9 @@ def attn_paged(q, k_cache, v_cache, table, lens, cu, o=None, lse=None, algo=L.AL
     row per request is a decode step, ``max_depth`` rows a draft, more a prompt in chunks.
 
     Returns ``(o, lse)``: ``o`` like ``q`` and fp32 ``lse`` ``[heads, T]``.  Rows behind
-    ``cu[B]`` are not written; a row that sees no key gives 0 and ``-inf``."""
+    ``cu[B]`` are not written; a row that sees no key gives 0 and ``-inf``.  Keys and values
+    below ``lens[b]`` are finite (the value of a key that a row does not see yet is multiplied
+    by its probability, 0); what lies behind them does not matter."""
     return _attn_paged(q, k_cache, v_cache, table, lens, cu, 0, o, lse, algo)
 
 
