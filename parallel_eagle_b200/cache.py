@@ -122,12 +122,13 @@ class DraftCache:
     def drop_prefix(self) -> None:
         """Give the shared prefix's pages back, for another one or none; every request has to
         be finished."""
+        if not self.shared:
+            return
         if any(n != self.shared for n in self.lengths):
             raise ValueError(f"the shared prefix of {self.shared} keys is dropped once every "
                              f"request is finished, not at lengths {self.lengths}")
-        if self.shared:
-            # its pages become request 0's own, which gives them back once
-            self.lens[1:].zero_()
-            self.lengths[1:] = [0] * (self.requests - 1)
-            self.shared = 0
-            self.resize([0] * self.requests)
+        # its pages become request 0's own, which gives them back once
+        self.lens[1:].zero_()
+        self.lengths[1:] = [0] * (self.requests - 1)
+        self.shared = 0
+        self.resize([0] * self.requests)

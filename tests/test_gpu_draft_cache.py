@@ -215,6 +215,8 @@ def test_prefixes_one_after_another():
         _check_pages(cache)
     have = [0] * 3
     _round(model, cache, seqs, have, [40, 7, 20], 4, tol)  # and without one
+    cache.drop_prefix()  # there is none
+    assert cache.lengths == [40, 7, 20]
     _check_pages(cache)
 
 
